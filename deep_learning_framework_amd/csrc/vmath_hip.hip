@@ -149,3 +149,31 @@ void VMath::attention_backward(int device, float* pgQ, float* pgK, float* pgV, f
 void VMath::dense_backward(int device, float* pgx, float* pgw, float* pgb, float* pga_work, float* pgy, float* pw, float* px, float* ppre, int64 yvec, int64 ndat, int64 xvec, int actFunc, HYPER h, bool acc) {
     raise_on(kai_dense_backward(device, pgx, pgw, pgb, pga_work, pgy, pw, px, ppre, yvec, ndat, xvec, actFunc, h, acc));
 }
+
+void VMath::rotary(int device, float* py, float* px, int* ppos, int64 nbat, int64 ntimes, int64 nvec, int64 nhead, int64 npiece, const kai_rotary_desc* desc) {
+    raise_on(kai_rotary(device, py, px, ppos, nbat, ntimes, nvec, nhead, npiece, desc));
+}
+
+void VMath::rotary_backward(int device, float* pgx, float* pgy, int* ppos, int64 nbat, int64 ntimes, int64 nvec, int64 nhead, int64 npiece, const kai_rotary_desc* desc) {
+    raise_on(kai_rotary_backward(device, pgx, pgy, ppos, nbat, ntimes, nvec, nhead, npiece, desc));
+}
+
+void VMath::cache_append(int device, float* pcK, float* pcV, float* pK, float* pV, int* ppage, int* plen, int* pcount, int* ppos, int64 nbat, int64 ntimes, int64 nvec,
+                         int64 nkvhead, int64 npiece, int64 npage, int64 npagelen, int64 nmaxpage, const kai_rotary_desc* desc) {
+    raise_on(kai_cache_append(device, pcK, pcV, pK, pV, ppage, plen, pcount, ppos, nbat, ntimes, nvec, nkvhead, npiece, npage, npagelen, nmaxpage, desc));
+}
+
+void VMath::cache_attention(int device, float* py, float* pQ, float* pcK, float* pcV, int* ppage, int* plen, int* pcount, int* pmask, int64 nbat, int64 ntimes, int64 nvec,
+                            int64 nhead, int64 nkvhead, int64 npiece, int64 npage, int64 npagelen, int64 nmaxpage, HYPER hCoef) {
+    raise_on(kai_cache_attention(device, py, pQ, pcK, pcV, ppage, plen, pcount, pmask, nbat, ntimes, nvec, nhead, nkvhead, npiece, npage, npagelen, nmaxpage, hCoef));
+}
+
+void VMath::gated_forward(int device, float* py, float* pgate, float* pup, float* pwg, float* pwu, float* pbg, float* pbu, float* px, int64 yvec, int64 ndat, int64 xvec,
+                          int actFunc, HYPER h) {
+    raise_on(kai_gated_forward(device, py, pgate, pup, pwg, pwu, pbg, pbu, px, yvec, ndat, xvec, actFunc, h));
+}
+
+void VMath::gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgbg, float* pgbu, float* pga_work, float* pgy, float* pwg, float* pwu, float* px,
+                           float* pgate, float* pup, int64 yvec, int64 ndat, int64 xvec, int actFunc, HYPER h, bool acc) {
+    raise_on(kai_gated_backward(device, pgx, pgwg, pgwu, pgbg, pgbu, pga_work, pgy, pwg, pwu, px, pgate, pup, yvec, ndat, xvec, actFunc, h, acc));
+}

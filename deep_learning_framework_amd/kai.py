@@ -87,10 +87,35 @@ SIGNATURES = {
     "kai_apply_decay": [_INT, _F, _F, _F, _I64, _F, _F],
     "kai_eval_adam_delta": [_INT, _F, _F, _F, _F, _F, _I64, _F, _F, _F],
     "kai_dense_backward": [_INT, _F, _F, _F, _F, _F, _F, _F, _F, _I64, _I64, _I64, _INT, _F, _INT],
+    "kai_rotary": [_INT, _F, _F, _F, _I64, _I64, _I64, _I64, _I64, _F],
+    "kai_rotary_backward": [_INT, _F, _F, _F, _I64, _I64, _I64, _I64, _I64, _F],
+    "kai_cache_append": [_INT] + [_F] * 8 + [_I64] * 8 + [_F],
+    "kai_cache_attention": [_INT] + [_F] * 8 + [_I64] * 9 + [_F],
+    "kai_gated_forward": [_INT] + [_F] * 8 + [_I64] * 3 + [_INT, _F],
+    "kai_gated_backward": [_INT] + [_F] * 12 + [_I64] * 3 + [_INT, _F, _INT],
 }
 
 ACT = {"none": 0, "relu": 1, "leaky": 2, "sigmoid": 3, "tanh": 4, "gelu": 5, "selu": 6, "mish": 7, "swish": 8,
        "softmax": 9}
+
+ROTARY_LAYOUT = {"halves": 0, "pairs": 1}
+ROTARY_SCALING = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+class RotaryDesc(ctypes.Structure):
+    """kai_rotary_desc: how positions turn the heads (host memory, read during a call)."""
+
+    _fields_ = [("nrot", ctypes.c_int64), ("layout", ctypes.c_int32), ("scaling", ctypes.c_int32)] + [
+        (n, ctypes.c_double) for n in ("base", "factor", "trained", "low_turns", "high_turns", "magnitude")]
+
+
+def rotary_desc(nrot, layout="halves", base=10000.0, scaling="none", factor=1.0, trained=0.0, low_turns=1.0,
+                high_turns=4.0, magnitude=1.0):
+    """A RotaryDesc: ``nrot`` elements at the front of a head turn, in ``layout`` "halves" or "pairs", with frequencies
+    ``base ** (-2 i / nrot)`` scaled as "none", "linear", "base" or "parts" says."""
+    return RotaryDesc(nrot, ROTARY_LAYOUT[layout], ROTARY_SCALING[scaling], base, factor, trained, low_turns, high_turns,
+                      magnitude)
+
 
 _lib = None
 
@@ -136,6 +161,10 @@ def _addr(p):
     if isinstance(p, DeviceBuffer):
         return p.ptr
     return int(p)
+
+
+def _desc(desc):
+    return None if desc is None else ctypes.addressof(desc)
 
 
 class DeviceBuffer:
@@ -463,3 +492,43 @@ class VMath:
         _ck(load().kai_dense_backward(device, _addr(pgx), _addr(pgw), _addr(pgb), _addr(pga_work), _addr(pgy),
                                       _addr(pw), _addr(px), _addr(ppre), yvec, ndat, xvec, actFunc,
                                       _addr(hLeakyAlpha), int(acc)))
+
+    # a decoder block: rotary positions, the cache of keys and values, the gated feed-forward projection
+    @staticmethod
+    def rotary(device, py, px, ppos, nbat, ntimes, nvec, nhead, npiece, desc):
+        """Turn the heads of px by their tokens' positions; ``desc`` is a ``rotary_desc(...)``."""
+        _ck(load().kai_rotary(device, _addr(py), _addr(px), _addr(ppos), nbat, ntimes, nvec, nhead, npiece, _desc(desc)))
+
+    @staticmethod
+    def rotary_backward(device, pgx, pgy, ppos, nbat, ntimes, nvec, nhead, npiece, desc):
+        _ck(load().kai_rotary_backward(device, _addr(pgx), _addr(pgy), _addr(ppos), nbat, ntimes, nvec, nhead, npiece,
+                                       _desc(desc)))
+
+    @staticmethod
+    def cache_append(device, pcK, pcV, pK, pV, ppage, plen, pcount, ppos, nbat, ntimes, nvec, nkvhead, npiece, npage,
+                     npagelen, nmaxpage, desc):
+        """Write new keys (turned by ``desc``, None: as they are) and values behind those of the cache."""
+        _ck(load().kai_cache_append(device, _addr(pcK), _addr(pcV), _addr(pK), _addr(pV), _addr(ppage), _addr(plen),
+                                    _addr(pcount), _addr(ppos), nbat, ntimes, nvec, nkvhead, npiece, npage, npagelen,
+                                    nmaxpage, _desc(desc)))
+
+    @staticmethod
+    def cache_attention(device, py, pQ, pcK, pcV, ppage, plen, pcount, pmask, nbat, ntimes, nvec, nhead, nkvhead, npiece,
+                        npage, npagelen, nmaxpage, hCoef):
+        """Attention of new tokens (a drafted tree with visibility words ``pmask``, or a run of tokens) over the cache."""
+        _ck(load().kai_cache_attention(device, _addr(py), _addr(pQ), _addr(pcK), _addr(pcV), _addr(ppage), _addr(plen),
+                                       _addr(pcount), _addr(pmask), nbat, ntimes, nvec, nhead, nkvhead, npiece, npage,
+                                       npagelen, nmaxpage, _addr(hCoef)))
+
+    @staticmethod
+    def gated_forward(device, py, pgate, pup, pwg, pwu, pbg, pbu, px, yvec, ndat, xvec, actFunc, hLeakyAlpha):
+        """py = act(px . pwg^T + pbg) * (px . pwu^T + pbu)."""
+        _ck(load().kai_gated_forward(device, _addr(py), _addr(pgate), _addr(pup), _addr(pwg), _addr(pwu), _addr(pbg),
+                                     _addr(pbu), _addr(px), yvec, ndat, xvec, actFunc, _addr(hLeakyAlpha)))
+
+    @staticmethod
+    def gated_backward(device, pgx, pgwg, pgwu, pgbg, pgbu, pga_work, pgy, pwg, pwu, px, pgate, pup, yvec, ndat, xvec,
+                       actFunc, hLeakyAlpha, acc):
+        _ck(load().kai_gated_backward(device, _addr(pgx), _addr(pgwg), _addr(pgwu), _addr(pgbg), _addr(pgbu),
+                                      _addr(pga_work), _addr(pgy), _addr(pwg), _addr(pwu), _addr(px), _addr(pgate),
+                                      _addr(pup), yvec, ndat, xvec, actFunc, _addr(hLeakyAlpha), int(acc)))

@@ -10,6 +10,8 @@ lists exactly as the reference's ``VTensor`` methods do and issue the same seque
 * ``mh_attention`` / ``mh_attention_backprop`` -- api_objects/vtensor.cpp:2978-3227
 * ``rnn`` / ``rnn_backprop`` (module level)  -- api_objects/vtensor.cpp:2350-2522, 2524-2717
 
+Additive, without a counterpart there: ``rotate``, ``gated`` / ``gated_backprop`` and ``KeyValueCache`` (a decoder block).
+
 Shape errors raise ``KaiError`` with the reference's codes (VERR_BAD_SHAPE_TENSOR = 10003).
 The graph, autograd queue and tracer of the engine are not rebuilt: backprop methods
 return the gradients instead of registering them in a queue.
@@ -140,9 +142,10 @@ class Tensor:
 
     # ---- mh_attention: vtensor.cpp:2978-3052 ----------------------------------------------------------
     def mh_attention(self, key, query, value, Kw, Kb, Qw, Qb, Vw, Vb, Ow, Ob, head_cnt, mask=False, coef=None,
-                     fused=False):
+                     fused=False, rotary=None):
         """``fused=False`` issues the reference's calls one by one; ``fused=True`` replaces the middle of the block
-        (mult_on_heads, mask, softmax_direct_on_axis, mix_values) by one kai_attention_forward_train."""
+        (mult_on_heads, mask, softmax_direct_on_axis, mix_values) by one kai_attention_forward_train.  ``rotary`` (a
+        kai.rotary_desc, additive) turns the projected keys and queries by their positions in place."""
         x = self
         if len(x.shape) != 3 or x.shape[2] % head_cnt != 0:
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "mh_attention")
@@ -171,6 +174,9 @@ class Tensor:
         VMath.add_bias(dev, K.ptr, K.ptr, Kb.ptr, n, nvec)
         VMath.add_bias(dev, Q.ptr, Q.ptr, Qb.ptr, n, nvec)
         VMath.add_bias(dev, V.ptr, V.ptr, Vb.ptr, n, nvec)
+        if rotary is not None:
+            rotate(K, nhead, rotary, out=K)
+            rotate(Q, nhead, rotary, out=Q)
         if fused:
             VMath.attention_forward_train(dev, mixed.ptr, probs.ptr, Q.ptr, K.ptr, V.ptr, nbat, ntimes, nvec, nhead,
                                           npiece, hcoef, mask)
@@ -184,7 +190,7 @@ class Tensor:
         VMath.add_bias(dev, y.ptr, y.ptr, Ob.ptr, n, nvec)
         y.saved = {"op": "mh_attention", "x": x, "key": key, "query": query, "value": value, "Kw": Kw, "Qw": Qw, "Vw": Vw,
                    "Ow": Ow, "K": K, "Q": Q, "V": V, "probs": probs, "mixed": mixed, "head_cnt": nhead,
-                   "mask": mask, "coef": hcoef}
+                   "mask": mask, "coef": hcoef, "rotary": rotary}
         return y
 
     # vtensor.cpp:3054-3195 (the math calls; gradient registration is the engine's business)
@@ -224,6 +230,9 @@ class Tensor:
                 VMath.set_mh_attention_mask(dev, g["probs"].ptr, nbat, ntimes, nhead, False)
             VMath.mult_on_heads_backward(dev, g["K"].ptr, g["probs"].ptr, s["Q"].ptr, nbat, ntimes, nvec, nhead, npiece)
             VMath.mult_on_heads_backward(dev, g["Q"].ptr, g["probs"].ptr, s["K"].ptr, nbat, ntimes, nvec, nhead, npiece)
+        if s["rotary"] is not None:
+            rotate(g["K"], nhead, s["rotary"], back=True, out=g["K"])
+            rotate(g["Q"], nhead, s["rotary"], back=True, out=g["Q"])
         VMath.add_bias_backward_b(dev, g["Kb"].ptr, g["K"].ptr, n, nvec, False)
         VMath.add_bias_backward_b(dev, g["Qb"].ptr, g["Q"].ptr, n, nvec, False)
         VMath.add_bias_backward_b(dev, g["Vb"].ptr, g["V"].ptr, n, nvec, False)
@@ -432,3 +441,99 @@ def rnn_backprop(saved, ygrad, ytgrad, use_state=False):
         VMath.matmul_backward_x(dev, pgx, aigrad.ptr, wi.ptr, ngates * nrec, ndat, ninp, False)
         VMath.matmul_backward_x(dev, pgr, argrad.ptr, wr.ptr, ngates * nrec, ndat, nrec, is_gru)
     return out
+
+
+# ---- the gated feed-forward projection (additive) ---------------------------------------------------------
+
+def gated(x, wg, wu, bg=None, bu=None, actfunc="swish", leaky_alpha=None, keep=False):
+    """activate(x . wg^T + bg) * (x . wu^T + bu) in one call; ``keep`` stores what ``gated_backprop`` reads."""
+    if len(wg.shape) != 2 or wg.shape != wu.shape or x.shape[-1] != wg.shape[1]:
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, "gated")
+    for b in (bg, bu):
+        if b is not None and b.total_size() != wg.shape[0]:
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, "gated")
+    yvec, xvec = wg.shape
+    ndat = x.total_size() // xvec
+    code = ACT[actfunc] if isinstance(actfunc, str) else int(actfunc)
+    h = kai.hyper(leaky_alpha, x.device)
+    y = Tensor(x.shape[:-1] + (yvec,), x.device)
+    gate, up = (Tensor(y.shape, x.device), Tensor(y.shape, x.device)) if keep else (None, None)
+    ptr = lambda t: t.ptr if t is not None else None
+    VMath.gated_forward(x.device, y.ptr, ptr(gate), ptr(up), wg.ptr, wu.ptr, ptr(bg), ptr(bu), x.ptr, yvec, ndat, xvec,
+                        code, h)
+    if keep:
+        y.saved = {"op": "gated", "x": x, "wg": wg, "wu": wu, "bg": bg, "bu": bu, "gate": gate, "up": up, "actfunc": code,
+                   "leaky_alpha": h}
+    return y
+
+
+def gated_backprop(y, ygrad):
+    """The gradients of ``gated`` by name: x, wg, wu and, where there are biases, bg and bu."""
+    s = y.saved
+    yvec, xvec = s["wg"].shape
+    ndat = s["x"].total_size() // xvec
+    dev = y.device
+    g = {name: Tensor(s[name].shape, dev) for name in ("x", "wg", "wu", "bg", "bu") if s[name] is not None}
+    ptr = lambda name: g[name].ptr if name in g else None
+    VMath.gated_backward(dev, ptr("x"), ptr("wg"), ptr("wu"), ptr("bg"), ptr("bu"), None, ygrad.ptr, s["wg"].ptr,
+                         s["wu"].ptr, s["x"].ptr, s["gate"].ptr, s["up"].ptr, yvec, ndat, xvec, s["actfunc"],
+                         s["leaky_alpha"], False)
+    return g
+
+
+# ---- a cache of keys and values (additive) -----------------------------------------------------------------
+
+class KeyValueCache:
+    """Pages of keys and values on the device, a table that finds each sequence's pages, and its length.
+
+    ``append`` writes the keys (turned by ``rotary``) and values of new tokens behind each sequence's own, ``attend``
+    lets the new tokens' queries see them, ``accept`` moves the lengths on: after a drafted tree only the tokens that
+    were taken, whose rows the caller has appended again in order where they did not stand first."""
+
+    def __init__(self, nbat, nkvhead, npiece, npagelen, nmaxpage, rotary=None, device=0):
+        self.nbat, self.nkvhead, self.npiece = nbat, nkvhead, npiece
+        self.npagelen, self.nmaxpage, self.npage = npagelen, nmaxpage, nbat * nmaxpage
+        self.rotary, self.device = rotary, device
+        shape = (self.npage, npagelen, nkvhead * npiece)
+        self.keys, self.values = Tensor(shape, device), Tensor(shape, device)
+        self.table = DeviceBuffer.from_numpy(np.arange(self.npage, dtype=np.int32).reshape(nbat, nmaxpage), device)
+        self.lengths = np.zeros(nbat, np.int32)
+        self._len = DeviceBuffer.from_numpy(self.lengths, device)
+
+    def accept(self, counts):
+        """Each sequence is ``counts`` (a number, or one per sequence) tokens longer."""
+        longer = self.lengths + np.asarray(counts, np.int32)
+        if np.any(longer < 0) or np.any(longer > self.npagelen * self.nmaxpage):
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, "accept")
+        self.lengths = longer.astype(np.int32)
+        self._len = DeviceBuffer.from_numpy(self.lengths, self.device)
+
+    def append(self, key, value, counts=None, positions=None):
+        if len(key.shape) != 3 or key.shape != value.shape or key.shape[0] != self.nbat or \
+                key.shape[2] != self.nkvhead * self.npiece:
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, "append")
+        VMath.cache_append(self.device, self.keys.ptr, self.values.ptr, key.ptr, value.ptr, self.table, self._len, counts,
+                           positions, self.nbat, key.shape[1], key.shape[2], self.nkvhead, self.npiece, self.npage,
+                           self.npagelen, self.nmaxpage, self.rotary)
+
+    def attend(self, query, head_cnt, counts=None, mask=None, coef=None):
+        if len(query.shape) != 3 or query.shape[0] != self.nbat or query.shape[2] != head_cnt * self.npiece:
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, "attend")
+        y = Tensor(query.shape, self.device)
+        VMath.set_zero(self.device, y.ptr, y.total_size() * 4)   # rows behind a sequence's count
+        hcoef = kai.hyper(1.0 / np.sqrt(self.npiece) if coef is None else coef, self.device)
+        VMath.cache_attention(self.device, y.ptr, query.ptr, self.keys.ptr, self.values.ptr, self.table, self._len, counts,
+                              mask, self.nbat, query.shape[1], query.shape[2], head_cnt, self.nkvhead, self.npiece,
+                              self.npage, self.npagelen, self.nmaxpage, hcoef)
+        return y
+
+
+def rotate(x, head_cnt, desc, positions=None, back=False, out=None):
+    """kai_rotary (``back``: kai_rotary_backward) of ``[nbat, ntimes, nvec]``; ``out`` may be ``x``."""
+    if len(x.shape) != 3 or x.shape[2] % head_cnt != 0:
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate")
+    nbat, ntimes, nvec = x.shape
+    y = out if out is not None else Tensor(x.shape, x.device)
+    call = VMath.rotary_backward if back else VMath.rotary
+    call(x.device, y.ptr, x.ptr, positions, nbat, ntimes, nvec, head_cnt, nvec // head_cnt, desc)
+    return y

@@ -388,6 +388,94 @@ int kai_attention_backward(int device, float* pgQ, float* pgK, float* pgV, const
                            int64_t ntimes, int64_t nvec, int64_t nhead, int64_t npiece, const float* hCoef,
                            int masked);
 
+/* ---- a decoder block: rotary positions, a cache of keys and values, the gated feed-forward projection ---- */
+/* Additive: the reference has no counterpart.  Same conventions as above (fp32, row-major, the calling thread's
+ * stream and device, nothing kept between calls). */
+
+#define KAI_ROTARY_HALVES 0   /* elements i and i + nrot/2 of a head turn together */
+#define KAI_ROTARY_PAIRS 1    /* elements 2i and 2i + 1 */
+
+#define KAI_ROTARY_SCALE_NONE 0
+#define KAI_ROTARY_SCALE_LINEAR 1   /* f_i / factor */
+#define KAI_ROTARY_SCALE_BASE 2     /* base * factor^(nrot / (nrot - 2)): the slowest pair turns `factor` times slower,
+                                       the fastest as before (nrot = 2 has one pair and stays as it is) */
+#define KAI_ROTARY_SCALE_PARTS 3    /* f_i (keep + (1 - keep) / factor), keep = clamp((turns_i - low_turns) /
+                                       (high_turns - low_turns), 0, 1), turns_i = trained f_i / 2 pi */
+
+/* How positions turn the heads, host memory, read during the call.  Pair i of the nrot rotated elements at the front
+ * of a head (0 <= nrot <= npiece, even, at most 512) turns by f_i = base^(-2i / nrot) radians a position, scaled for
+ * contexts longer than the trained one; cosine and sine are multiplied by `magnitude`.  Fields that a scaling does
+ * not name are not read. */
+typedef struct kai_rotary_desc {
+    int64_t nrot;
+    int32_t layout;
+    int32_t scaling;
+    double base;
+    double factor;
+    double trained;
+    double low_turns;
+    double high_turns;
+    double magnitude;
+} kai_rotary_desc;
+
+/* Turns the heads of px[nbat, ntimes, nvec] (head h at h * npiece, nhead * npiece <= nvec, at most 2^24) by their
+ * tokens' positions: y1 = m (x1 cos - x2 sin), y2 = m (x2 cos + x1 sin) for the two elements of a pair; the elements
+ * of a head behind nrot are copied.  ppos[nbat, ntimes] holds the positions (any int, angles formed in 64 bits), null:
+ * 0 .. ntimes - 1.  py has px's layout; columns behind nhead * npiece are left as they are.  py may equal px; buffers
+ * that overlap otherwise are not supported.  Goes between the projections and kai_mult_on_heads /
+ * kai_attention_forward(_train). */
+int kai_rotary(int device, float* py, const float* px, const int* ppos, int64_t nbat, int64_t ntimes, int64_t nvec,
+               int64_t nhead, int64_t npiece, const kai_rotary_desc* desc);
+/* Its gradient: pgy turned back by the same angles, times the magnitude.  pgx may equal pgy. */
+int kai_rotary_backward(int device, float* pgx, const float* pgy, const int* ppos, int64_t nbat, int64_t ntimes,
+                        int64_t nvec, int64_t nhead, int64_t npiece, const kai_rotary_desc* desc);
+
+/* The cache.  pcK and pcV are [npage, npagelen, nkvhead * npiece] each.  Key j of sequence b is row j % npagelen of
+ * page ppage[b, j / npagelen] (ppage[nbat, nmaxpage]; null: page b, nmaxpage <= 1, npage >= nbat).  A page number
+ * outside [0, npage) names no page: writes to it are dropped, its keys are not seen; nor are keys at nmaxpage *
+ * npagelen (below 2^31) and behind.  plen[nbat] is the number of keys a sequence holds already (negative: 0); the new
+ * ones stand behind it.  pcount[nbat], or null for ntimes, is how many of the ntimes rows of a sequence are new tokens
+ * (clipped to 0 .. ntimes): the rows behind it are not read, and their results are left as they were. */
+
+/* Writes the keys pK and values pV[nbat, ntimes, nvec] (head h at h * npiece, nkvhead * npiece <= nvec) of the new tokens
+ * behind the sequences' own, the keys turned on the way as kai_rotary does (desc null: not turned) by the positions
+ * ppos[nbat, ntimes], null: plen[b] + t.  plen is not changed.  No two tokens of a call may have the same row: of
+ * sequences that share a page only one may write there. */
+int kai_cache_append(int device, float* pcK, float* pcV, const float* pK, const float* pV, const int* ppage,
+                     const int* plen, const int* pcount, const int* ppos, int64_t nbat, int64_t ntimes, int64_t nvec,
+                     int64_t nkvhead, int64_t npiece, int64_t npage, int64_t npagelen, int64_t nmaxpage,
+                     const kai_rotary_desc* desc);
+
+/* Attention of the new tokens over the cache, which holds their own keys too (kai_cache_append):
+ *   py[b, t, h, :] = sum_j softmax_j(coef <q, k_j>) v_j over the keys j that row (b, t) sees: every key in front of
+ * plen[b], and of the new tokens those whose bit is set: new token s is bit s % 32 of word pmask[b, t, s / 32] (ntimes
+ * bits a row, in ceil(ntimes / 32) words), so that a drafted tree's node sees its ancestors and itself.  pmask null:
+ * s <= t.  One new token is a step of plain decoding.  pQ is [nbat, ntimes, nvec] (head h at h * npiece, nhead * npiece <=
+ * nvec), py[nbat, ntimes, nhead * npiece]; head h reads the keys of head h / (nhead / nkvhead) (nkvhead divides nhead).
+ * npiece is at most 256.  A row that sees no key, or none whose score is above minus infinity, gives zeros; what
+ * stands at keys that a row does not see (NaN included) does not reach it.  The keys are cut into parts whose
+ * results meet in the library scratch. */
+int kai_cache_attention(int device, float* py, const float* pQ, const float* pcK, const float* pcV, const int* ppage,
+                        const int* plen, const int* pcount, const int* pmask, int64_t nbat, int64_t ntimes, int64_t nvec,
+                        int64_t nhead, int64_t nkvhead, int64_t npiece, int64_t npage, int64_t npagelen, int64_t nmaxpage,
+                        const float* hCoef);
+
+/* The gated feed-forward projection: py[ndat, yvec] = act(px . pwg^T + pbg) * (px . pwu^T + pbu), pwg and pwu
+ * [yvec, xvec], the biases [yvec] or null, activation codes 0..8.  pgate and pup (both or neither) receive the two sums
+ * in front of the activation and the product, which kai_gated_backward reads.  The outputs overlap neither one another
+ * nor the inputs. */
+int kai_gated_forward(int device, float* py, float* pgate, float* pup, const float* pwg, const float* pwu,
+                      const float* pbg, const float* pbu, const float* px, int64_t yvec, int64_t ndat, int64_t xvec,
+                      int actFunc, const float* hLeakyAlpha);
+/* Its gradients: with gg = pgy * up * act'(gate) and gu = pgy * act(gate),
+ *   pgx = gg . wg + gu . wu,  pgwg = gg^T . x,  pgwu = gu^T . x,  pgbg, pgbu = column sums of gg, gu
+ * (+= where acc != 0); any of the five may be null.  pga_work receives gg and gu: a buffer of 2 * ndat * yvec floats,
+ * or null for the library scratch. */
+int kai_gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgbg, float* pgbu, float* pga_work,
+                       const float* pgy, const float* pwg, const float* pwu, const float* px, const float* pgate,
+                       const float* pup, int64_t yvec, int64_t ndat, int64_t xvec, int actFunc, const float* hLeakyAlpha,
+                       int acc);
+
 #ifdef __cplusplus
 }
 #endif

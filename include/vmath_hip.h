@@ -35,6 +35,8 @@ private:
     int m_code;
 };
 
+struct kai_rotary_desc;   /* kai_hip.h */
+
 class VMath {
 public:
     static void* mem_alloc(int device, int64 size);
@@ -104,6 +106,18 @@ public:
     static void attention_backward(int device, float* pgQ, float* pgK, float* pgV, float* pgm, float* pp, float* pm, float* pQ, float* pK, float* pV, int64 nbat, int64 ntimes, int64 nvec, int64 nhead, int64 npiece, HYPER hCoef, bool masked);
     static void dense_forward(int device, float* py, float* ppre, float* pw, float* pb, float* px, int64 yvec, int64 ndat, int64 xvec, int actFunc, HYPER hLeakyAlpha);
     static void dense_backward(int device, float* pgx, float* pgw, float* pgb, float* pga_work, float* pgy, float* pw, float* px, float* ppre, int64 yvec, int64 ndat, int64 xvec, int actFunc, HYPER hLeakyAlpha, bool acc);
+
+    // additive: a decoder block (see kai_rotary, kai_cache_append, kai_cache_attention, kai_gated_forward)
+    static void rotary(int device, float* py, float* px, int* ppos, int64 nbat, int64 ntimes, int64 nvec, int64 nhead, int64 npiece, const kai_rotary_desc* desc);
+    static void rotary_backward(int device, float* pgx, float* pgy, int* ppos, int64 nbat, int64 ntimes, int64 nvec, int64 nhead, int64 npiece, const kai_rotary_desc* desc);
+    static void cache_append(int device, float* pcK, float* pcV, float* pK, float* pV, int* ppage, int* plen, int* pcount, int* ppos, int64 nbat, int64 ntimes, int64 nvec,
+                             int64 nkvhead, int64 npiece, int64 npage, int64 npagelen, int64 nmaxpage, const kai_rotary_desc* desc);
+    static void cache_attention(int device, float* py, float* pQ, float* pcK, float* pcV, int* ppage, int* plen, int* pcount, int* pmask, int64 nbat, int64 ntimes, int64 nvec,
+                                int64 nhead, int64 nkvhead, int64 npiece, int64 npage, int64 npagelen, int64 nmaxpage, HYPER hCoef);
+    static void gated_forward(int device, float* py, float* pgate, float* pup, float* pwg, float* pwu, float* pbg, float* pbu, float* px, int64 yvec, int64 ndat, int64 xvec,
+                              int actFunc, HYPER hLeakyAlpha);
+    static void gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgbg, float* pgbu, float* pga_work, float* pgy, float* pwg, float* pwu, float* px,
+                               float* pgate, float* pup, int64 yvec, int64 ndat, int64 xvec, int actFunc, HYPER hLeakyAlpha, bool acc);
 };
 
 #endif

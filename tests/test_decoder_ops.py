@@ -1,0 +1,795 @@
+"""The operators of a decoder block against plain implementations in 64 bits: rotary positions, the cache of keys and
+values, attention of new tokens over it, the gated feed-forward projection, their refusals and a run of them together.
+
+Tolerances (fp32, half a step 2^-24 relative to a value):
+* rotary: the turn's fraction is rounded once (below 1/2: 2^-26 absolute, 2 pi 2^-26 < 1.6 * 2^-24 rad), sine and cosine are
+  good to 2 steps, the magnitude, each of the two products and the sum round once: below 10 * 2^-24 of m (|x1| + |x2|);
+* attention: a score of d products is off by (d + 2) 2^-24 of coef sum |q k|; twice the largest such error, and one rounding
+  for each key of the two sums, reach the result, relative to the largest |v|;
+* the gated projection: the repository's relative Frobenius 1e-5 for sums in another order."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from util import REL_FRO_TOL, rel_fro
+
+from deep_learning_framework_amd import kai
+from deep_learning_framework_amd.kai import ACT, DeviceBuffer, KaiError, VMath
+from deep_learning_framework_amd.tensor_ops import (KeyValueCache, Tensor, gated, gated_backprop, rotate)
+
+HALF_STEP = 2.0 ** -24
+dev_int = lambda a: DeviceBuffer.from_numpy(np.asarray(a, np.int32))
+
+
+# ---- plain implementations in 64 bits ----------------------------------------------------------------------------
+
+def plain_frequencies(d):
+    half = d.nrot // 2
+    i = np.arange(half)
+    base = d.base
+    if d.scaling == 2 and d.nrot > 2:
+        base = base * d.factor ** (d.nrot / (d.nrot - 2))
+    f = base ** (-2.0 * i / d.nrot)
+    if d.scaling == 1:
+        f = f / d.factor
+    if d.scaling == 3:
+        turns = d.trained * f / (2 * np.pi)
+        keep = np.clip((turns - d.low_turns) / (d.high_turns - d.low_turns), 0, 1)
+        f = f * keep + f / d.factor * (1 - keep)
+    return f
+
+
+def plain_rotary(x, pos, d, back=False):
+    """x [..., heads, npiece] with positions [...]"""
+    x = np.asarray(x, np.float64)
+    half = d.nrot // 2
+    angle = np.asarray(pos, np.float64)[..., None] * plain_frequencies(d)
+    c, s = (d.magnitude * f(angle)[..., None, :] for f in (np.cos, np.sin))
+    s = -s if back else s
+    first = np.arange(half) if d.layout == 0 else 2 * np.arange(half)
+    second = first + half if d.layout == 0 else first + 1
+    y = x.copy()
+    y[..., first] = x[..., first] * c - x[..., second] * s
+    y[..., second] = x[..., second] * c + x[..., first] * s
+    room = np.zeros_like(y)
+    room[..., first] = room[..., second] = abs(d.magnitude) * (np.abs(x[..., first]) + np.abs(x[..., second]))
+    return y, room
+
+
+def plain_attention(q, keys, values, see, coef):
+    """q [t, h, d], keys / values [n, kv, d], see [t, n] -> [t, h, d] and how far a 32-bit result may be off"""
+    q, keys, values = (np.asarray(a, np.float64) for a in (q, keys, values))
+    t, h, d = q.shape
+    group = h // keys.shape[1]
+    y, room = np.zeros((t, h, d)), np.zeros((t, h, d))
+    for i in range(t):
+        js = np.flatnonzero(see[i])
+        for j in range(h):
+            if len(js) == 0:
+                continue
+            k, v = keys[js, j // group], values[js, j // group]
+            z = coef * (k @ q[i, j])
+            p = np.exp(z - z.max())
+            y[i, j] = (p / p.sum()) @ v
+            off = (d + 2) * HALF_STEP * abs(coef) * (np.abs(k) @ np.abs(q[i, j])).max()
+            room[i, j] = np.abs(v).max() * (2 * np.expm1(off) + (len(js) + 12) * HALF_STEP)
+    return y, room
+
+
+def words_of(see):
+    """[t, t] visibility of new tokens -> [t, ceil(t / 32)] words"""
+    t = see.shape[0]
+    w = np.zeros((t, (t + 31) // 32), np.uint32)
+    for i in range(t):
+        for j in np.flatnonzero(see[i]):
+            w[i, j // 32] |= np.uint32(1) << np.uint32(j % 32)
+    return w.view(np.int32)
+
+
+def random_tree(rng, t):
+    see = np.zeros((t, t), bool)
+    for i in range(t):
+        if i:
+            see[i] = see[rng.integers(0, i)]
+        see[i, i] = True
+    return see
+
+
+ACTS = {
+    "none": (lambda g: g, lambda g: np.ones_like(g)),
+    "relu": (lambda g: np.maximum(g, 0), lambda g: (g > 0) * 1.0),
+    "leaky": (lambda g: np.where(g > 0, g, 0.25 * g), lambda g: np.where(g > 0, 1.0, 0.25)),
+    "sigmoid": (lambda g: 1 / (1 + np.exp(-g)), lambda g: np.exp(-g) / (1 + np.exp(-g)) ** 2),
+    "tanh": (np.tanh, lambda g: 1 - np.tanh(g) ** 2),
+    "swish": (lambda g: g / (1 + np.exp(-g)),
+              lambda g: 1 / (1 + np.exp(-g)) + g * np.exp(-g) / (1 + np.exp(-g)) ** 2),
+}
+
+
+def _gelu():
+    from math import erf, pi, sqrt
+    cdf = np.vectorize(lambda g: 0.5 * (1 + erf(g / sqrt(2))))
+    ACTS["gelu"] = (lambda g: g * cdf(g), lambda g: cdf(g) + g * np.exp(-g * g / 2) / sqrt(2 * pi))
+
+
+_gelu()
+
+
+# ---- refusals (no GPU) -------------------------------------------------------------------------------------------
+
+def _refused(code, call, *args):
+    with pytest.raises(KaiError) as e:
+        call(*args)
+    assert e.value.code == code, e.value.message
+
+
+ONE = 4096   # a non-null address that a refused call never reads
+
+
+def test_rotary_refusals():
+    d = kai.rotary_desc(8)
+    ok = (ONE, ONE, None, 2, 3, 16, 2, 8)
+    for call in (VMath.rotary, VMath.rotary_backward):
+        _refused(510, call, -1, *ok, d)
+        _refused(523, call, 0, *ok, None)
+        _refused(523, call, 0, None, *ok[1:], d)
+        _refused(523, call, 0, ONE, None, *ok[2:], d)
+        _refused(510, call, 0, ONE, ONE, None, 2, 3, 15, 2, 8, d)           # heads wider than the row
+        _refused(510, call, 0, ONE, ONE, None, -1, 3, 16, 2, 8, d)
+        _refused(510, call, 0, ONE, ONE, None, 2 ** 20, 2 ** 20, 16, 2, 8, d)   # too many tokens
+        _refused(510, call, 0, ONE, ONE, None, 1, 1, 2 ** 25, 1, 2 ** 25, d)    # too wide
+        for bad in (kai.rotary_desc(7), kai.rotary_desc(10), kai.rotary_desc(-2), kai.rotary_desc(8, base=0.0),
+                    kai.rotary_desc(8, base=float("nan")), kai.rotary_desc(8, magnitude=float("inf")),
+                    kai.rotary_desc(8, scaling="linear", factor=0.0), kai.rotary_desc(8, scaling="base", factor=-1.0),
+                    kai.rotary_desc(8, scaling="parts", factor=2.0, trained=0.0),
+                    kai.rotary_desc(8, scaling="parts", factor=2.0, trained=10.0, low_turns=4.0, high_turns=4.0)):
+            _refused(510, call, 0, *ok, bad)
+        odd = kai.rotary_desc(8)
+        odd.layout = 2
+        _refused(510, call, 0, *ok, odd)
+        odd = kai.rotary_desc(8)
+        odd.scaling = 4
+        _refused(510, call, 0, *ok, odd)
+        _refused(510, call, 0, ONE, ONE, None, 1, 1, 2048, 1, 2048, kai.rotary_desc(514))
+        call(0, ONE, ONE, None, 0, 3, 16, 2, 8, d)                            # nothing to do
+        call(0, ONE, ONE, None, 2, 3, 16, 2, 8, kai.rotary_desc(0))           # in place, nothing turned
+
+
+def test_cache_refusals():
+    append = lambda dev=0, ck=ONE, cv=ONE, k=ONE, v=ONE, table=ONE, ln=ONE, nbat=2, nt=3, nvec=16, nkv=2, npc=8, npage=4, \
+        page=16, most=2, d=None: VMath.cache_append(dev, ck, cv, k, v, table, ln, None, None, nbat, nt, nvec, nkv, npc, npage,
+                                                    page, most, d)
+    attend = lambda dev=0, y=ONE, q=2 * ONE, ck=ONE, cv=ONE, table=ONE, ln=ONE, nbat=2, nt=3, nvec=32, nh=4, nkv=2, npc=8, \
+        npage=4, page=16, most=2: VMath.cache_attention(dev, y, q, ck, cv, table, ln, None, None, nbat, nt, nvec, nh, nkv,
+                                                        npc, npage, page, most, None)
+    for call in (append, attend):
+        _refused(510, lambda: call(dev=-1))
+        _refused(510, lambda: call(nbat=-1))
+        _refused(510, lambda: call(page=-1))
+        _refused(510, lambda: call(nvec=15))
+        _refused(510, lambda: call(page=2 ** 16, most=2 ** 16))
+        _refused(510, lambda: call(table=None))              # two pages a sequence need a table
+        _refused(510, lambda: call(table=None, most=1, npage=1))
+        _refused(523, lambda: call(ln=None))
+        _refused(523, lambda: call(ck=None))
+        _refused(523, lambda: call(cv=None))
+        call(nbat=0)
+        call(nt=0)
+    append(page=0)
+    append(npage=0)
+    _refused(510, lambda: append(d=kai.rotary_desc(10)))
+    _refused(523, lambda: append(k=None))
+    _refused(523, lambda: append(v=None))
+    _refused(510, lambda: attend(nkv=3))
+    _refused(510, lambda: attend(nkv=0))
+    _refused(510, lambda: attend(npc=257, nvec=257 * 4))
+    _refused(523, lambda: attend(y=None))
+    _refused(523, lambda: attend(q=None))
+    _refused(510, lambda: attend(y=ONE, q=ONE))
+
+
+def test_gated_refusals():
+    ok = dict(y=ONE, g=None, u=None, wg=ONE, wu=ONE, x=ONE, yvec=8, ndat=4, xvec=8, act=8, dev=0)
+
+    def forward(**k):
+        a = dict(ok, **k)
+        VMath.gated_forward(a["dev"], a["y"], a["g"], a["u"], a["wg"], a["wu"], None, None, a["x"], a["yvec"], a["ndat"],
+                            a["xvec"], a["act"], None)
+
+    for code, bad in ((510, dict(dev=-1)), (510, dict(yvec=-1)), (510, dict(xvec=2 ** 31)), (8, dict(act=9)), (8, dict(act=-1)),
+                      (523, dict(y=None)), (523, dict(wg=None)), (523, dict(wu=None)), (523, dict(x=None)),
+                      (523, dict(g=ONE)), (523, dict(u=ONE))):
+        _refused(code, lambda: forward(**bad))
+    forward(ndat=0)
+    forward(yvec=0)
+
+    def backward(**k):
+        a = dict(dict(gx=ONE, gwg=ONE, gwu=ONE, gb=None, gy=ONE, wg=ONE, wu=ONE, x=ONE, gate=ONE, up=ONE, act=8, dev=0, ndat=4),
+                 **k)
+        VMath.gated_backward(a["dev"], a["gx"], a["gwg"], a["gwu"], a["gb"], a["gb"], ONE, a["gy"], a["wg"], a["wu"], a["x"],
+                             a["gate"], a["up"], 8, a["ndat"], 8, a["act"], None, False)
+
+    for code, bad in ((510, dict(dev=-1)), (510, dict(ndat=-1)), (8, dict(act=9)), (523, dict(gy=None)),
+                      (523, dict(gate=None)), (523, dict(up=None)), (523, dict(wg=None)), (523, dict(wu=None)),
+                      (523, dict(x=None))):
+        _refused(code, lambda: backward(**bad))
+
+
+def test_structure_matches_header():
+    assert ctypes.sizeof(kai.RotaryDesc) == 64
+    assert kai.RotaryDesc.base.offset == 16 and kai.RotaryDesc.magnitude.offset == 56
+
+
+# ---- rotary ------------------------------------------------------------------------------------------------------
+
+ROTARY_CASES = [
+    # nbat, ntimes, nhead, npiece, extra columns, desc, positions
+    (2, 7, 3, 16, 0, dict(nrot=16), None),
+    (2, 7, 3, 16, 0, dict(nrot=16, layout="pairs"), None),
+    (1, 1, 1, 2, 0, dict(nrot=2), "far"),
+    (1, 1, 1, 2, 3, dict(nrot=2, scaling="base", factor=4.0), "far"),
+    (3, 5, 2, 10, 7, dict(nrot=6, layout="pairs", scaling="linear", factor=4.0), "far"),
+    (3, 5, 2, 10, 7, dict(nrot=6, scaling="base", factor=2.0), "far"),
+    (2, 33, 12, 64, 0, dict(nrot=64), "far"),
+    (2, 33, 12, 64, 128, dict(nrot=32, layout="pairs", scaling="parts", factor=8.0, trained=4096.0, magnitude=1.2), "far"),
+    (1, 3, 4, 128, 0, dict(nrot=128, base=500000.0, scaling="parts", factor=8.0, trained=8192.0, low_turns=1.0), "signed"),
+    (1, 300, 5, 24, 0, dict(nrot=24, layout="pairs"), None),
+    (1, 9000, 1, 8, 0, dict(nrot=8), None),
+    (4, 4, 2, 20, 0, dict(nrot=12), "far"),
+    (1, 2, 1, 600, 0, dict(nrot=512), "far"),
+    (2, 3, 2, 12, 0, dict(nrot=0), "far"),
+]
+
+
+def _positions(rng, kind, nbat, ntimes):
+    if kind is None:
+        return None, np.broadcast_to(np.arange(ntimes), (nbat, ntimes))
+    p = rng.integers(0, 1 << 20, (nbat, ntimes))
+    if kind == "signed":
+        p = rng.integers(-2 ** 31, 2 ** 31 - 1, (nbat, ntimes))
+    return dev_int(p), p
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("case", range(len(ROTARY_CASES)))
+def test_rotary(case, back):
+    nbat, ntimes, nhead, npiece, extra, desc, where = ROTARY_CASES[case]
+    rng = np.random.default_rng(case)
+    d = kai.rotary_desc(**desc)
+    nvec = nhead * npiece + extra
+    x = rng.standard_normal((nbat, ntimes, nvec)).astype(np.float32)
+    dpos, pos = _positions(rng, where, nbat, ntimes)
+    heads = x[..., :nhead * npiece].reshape(nbat, ntimes, nhead, npiece)
+    want, room = plain_rotary(heads, pos, d, back)
+    # at positions of 2^31 the 64-bit product itself is off by 2^-53 * 2^31 turns, in the plain form too
+    tol = 10 * HALF_STEP * room + (2.0 ** -20 * room if where == "signed" else 0)
+    call = VMath.rotary_backward if back else VMath.rotary
+    px = DeviceBuffer.from_numpy(x)
+    for off in (0, 1):          # aligned, and 4 bytes into a buffer
+        py = DeviceBuffer.from_numpy(np.full(x.size + off, 7.0, np.float32))
+        call(0, py.offset(4 * off), px, dpos, nbat, ntimes, nvec, nhead, npiece, d)
+        got = py.to_numpy(x.size + off)
+        assert np.all(got[:off] == 7.0)
+        got = got[off:].reshape(x.shape)
+        g = got[..., :nhead * npiece].reshape(heads.shape).astype(np.float64)
+        assert np.all(np.abs(g - want) <= tol)
+        assert np.all(got[..., nhead * npiece:] == 7.0), "columns behind the heads are not written"
+        assert np.array_equal(g[..., d.nrot:], heads[..., d.nrot:])
+    call(0, px, px, dpos, nbat, ntimes, nvec, nhead, npiece, d)   # in place: the same bits
+    inplace = px.to_numpy(x.shape)
+    assert np.array_equal(inplace[..., :nhead * npiece], got[..., :nhead * npiece])
+    assert np.array_equal(inplace[..., nhead * npiece:], x[..., nhead * npiece:])
+
+
+@pytest.mark.gpu
+def test_rotary_gradient_against_differences():
+    rng = np.random.default_rng(3)
+    d = kai.rotary_desc(12, layout="pairs", scaling="parts", factor=4.0, trained=64.0, magnitude=1.3)
+    shape = (2, 5, 3, 16)
+    pos = rng.integers(0, 500, shape[:2])
+    x, gy = rng.standard_normal(shape), rng.standard_normal(shape)
+    dpos = dev_int(pos)
+    t = Tensor.from_numpy(gy.reshape(2, 5, 48))
+    g = rotate(t, 3, d, positions=dpos, back=True).numpy().reshape(shape).astype(np.float64)
+    f = lambda v: np.sum(plain_rotary(v, pos, d)[0] * gy.astype(np.float32))
+    for k in range(20):
+        e = np.zeros(shape)
+        e[tuple(rng.integers(0, s) for s in shape)] = 1.0
+        diff = (f(x + 0.5 * e) - f(x - 0.5 * e))     # linear in x: a difference is the derivative
+        assert abs(np.sum(g * e) - diff) <= 20 * HALF_STEP * 1.3 * 2 * np.abs(gy).max()
+
+
+# ---- the cache ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("npiece,nkv,page,nrot,layout,extra", [(16, 2, 5, 16, "halves", 0), (12, 3, 8, 6, "pairs", 5),
+                                                               (64, 1, 16, 32, "halves", 64), (7, 2, 3, 4, "halves", 0),
+                                                               (8, 2, 4, 0, "halves", 0), (128, 8, 64, 128, "pairs", 0)])
+@pytest.mark.parametrize("given", [False, True])
+def test_cache_append(npiece, nkv, page, nrot, layout, extra, given):
+    rng = np.random.default_rng(npiece + page)
+    nbat, ntimes, most = 5, 9, 6
+    width, nvec = nkv * npiece, nkv * npiece + extra
+    npage = nbat * most + 2
+    table = rng.permutation(npage)[:nbat * most].reshape(nbat, most).astype(np.int32)
+    lens = np.array([0, 1, page * most - 4, -3, 2 * page - 1], np.int32)     # 2: runs out of pages, 3: read as 0
+    counts = np.array([9, 0, 9, 20, 4], np.int32)                            # 3: clipped to ntimes
+    table[4, 2] = -1                                                         # a page that does not exist
+    table[0, 1] = npage                                                      # nor this one
+    k, v = (rng.standard_normal((nbat, ntimes, nvec)).astype(np.float32) for _ in range(2))
+    k[1], v[4, 4:] = np.nan, np.nan                                          # rows behind the counts are not read
+    ck, cv = (rng.standard_normal((npage, page, width)).astype(np.float32) for _ in range(2))
+    pos = rng.integers(0, 100000, (nbat, ntimes)) if given else np.maximum(lens, 0)[:, None] + np.arange(ntimes)
+    d = kai.rotary_desc(nrot, layout=layout)
+    turned, room = plain_rotary(k[..., :width].reshape(nbat, ntimes, nkv, npiece), pos, d)
+    turned, room = turned.reshape(nbat, ntimes, width), room.reshape(nbat, ntimes, width)
+    wk, wv, tol = ck.astype(np.float64), cv.copy(), np.zeros(ck.shape)
+    for b in range(nbat):
+        for t in range(min(counts[b], ntimes)):
+            at = max(lens[b], 0) + t
+            if at >= page * most or not 0 <= table[b, at // page] < npage:
+                continue
+            p, r = table[b, at // page], at % page
+            wk[p, r], wv[p, r], tol[p, r] = turned[b, t], v[b, t, :width], 10 * HALF_STEP * room[b, t]
+    for off in (0, 1):
+        bk, bv = (DeviceBuffer.from_numpy(np.concatenate([np.zeros(off, np.float32), c.ravel()])) for c in (ck, cv))
+        VMath.cache_append(0, bk.offset(4 * off), bv.offset(4 * off), DeviceBuffer.from_numpy(k), DeviceBuffer.from_numpy(v),
+                           dev_int(table), dev_int(lens), dev_int(counts), dev_int(pos) if given else None, nbat, ntimes, nvec,
+                           nkv, npiece, npage, page, most, d if nrot or not given else None)
+        gk, gv = (b.to_numpy(ck.size + off)[off:].reshape(ck.shape) for b in (bk, bv))
+        assert np.all(np.abs(gk - wk) <= tol)
+        assert np.array_equal(gv, wv)
+
+
+# ---- attention over the cache -------------------------------------------------------------------------------------
+
+def _attention_case(rng, nbat, ntimes, nhead, nkv, npiece, page, lens, counts, tree, extra=0, scale=1.0):
+    most = max(1, -(-(max(max(l, 0) for l in lens) + ntimes) // page))
+    npage = nbat * most + 1
+    table = rng.permutation(npage)[:nbat * most].reshape(nbat, most).astype(np.int32)
+    width = nkv * npiece
+    ck, cv = (rng.standard_normal((npage, page, width)).astype(np.float32) for _ in range(2))
+    q = (scale * rng.standard_normal((nbat, ntimes, nhead * npiece + extra))).astype(np.float32)
+    see_new = np.stack([random_tree(rng, ntimes) if tree else np.tril(np.ones((ntimes, ntimes), bool)) for _ in range(nbat)])
+    return dict(nbat=nbat, ntimes=ntimes, nhead=nhead, nkv=nkv, npiece=npiece, page=page, most=most, npage=npage, table=table,
+                ck=ck, cv=cv, q=q, see_new=see_new, lens=np.asarray(lens, np.int32),
+                counts=None if counts is None else np.asarray(counts, np.int32), tree=tree, extra=extra)
+
+
+def _attend(c, q_off=0, c_off=0, coef=None, hold=None):
+    nvec = c["nhead"] * c["npiece"] + c["extra"]
+    coef = 1.0 / np.sqrt(c["npiece"]) if coef is None else coef
+    put = lambda a, off: DeviceBuffer.from_numpy(np.concatenate([np.zeros(off, np.float32), a.ravel()]))
+    q, ck, cv = put(c["q"], q_off), put(c["ck"], c_off), put(c["cv"], c_off)
+    size = c["nbat"] * c["ntimes"] * c["nhead"] * c["npiece"]
+    y = DeviceBuffer.from_numpy(np.full(size + q_off, 5.0, np.float32))
+    words = np.stack([words_of(s) for s in c["see_new"]]) if c["tree"] else None
+    VMath.cache_attention(0, y.offset(4 * q_off), q.offset(4 * q_off), ck.offset(4 * c_off), cv.offset(4 * c_off),
+                          dev_int(c["table"]), dev_int(c["lens"]), None if c["counts"] is None else dev_int(c["counts"]),
+                          None if words is None else dev_int(words), c["nbat"], c["ntimes"], nvec, c["nhead"], c["nkv"],
+                          c["npiece"], c["npage"], c["page"], c["most"], kai.hyper(coef))
+    return y.to_numpy(size + q_off)[q_off:].reshape(c["nbat"], c["ntimes"], c["nhead"], c["npiece"])
+
+
+def _expected(c, coef=None):
+    coef = float(np.float32(1.0 / np.sqrt(c["npiece"]) if coef is None else coef))
+    y = np.full((c["nbat"], c["ntimes"], c["nhead"], c["npiece"]), 5.0)
+    room = np.zeros(y.shape)
+    for b in range(c["nbat"]):
+        n = max(int(c["lens"][b]), 0)
+        count = c["ntimes"] if c["counts"] is None else min(max(int(c["counts"][b]), 0), c["ntimes"])
+        total = min(n + count, c["page"] * c["most"])
+        at = np.arange(total)
+        pages = c["table"][b, at // c["page"]]
+        exists = (pages >= 0) & (pages < c["npage"])
+        rows = np.where(exists, pages, 0), at % c["page"]
+        k, v = (c[s][rows].reshape(total, c["nkv"], c["npiece"]) for s in ("ck", "cv"))
+        see = np.ones((count, total), bool)
+        new = at[at >= n] - n
+        see[:, at >= n] = c["see_new"][b][:count][:, new]
+        see &= exists[None, :]
+        q = c["q"][b, :count, :c["nhead"] * c["npiece"]].reshape(count, c["nhead"], c["npiece"])
+        y[b, :count], room[b, :count] = plain_attention(q, k, v, see, coef)
+    return y, room
+
+
+def _check_attention(c, **k):
+    got = _attend(c, **k)
+    want, room = _expected(c, k.get("coef"))
+    bad = np.abs(got - want) > room
+    assert not bad.any(), "%d of %d off, worst %g at %s" % (
+        bad.sum(), bad.size, np.nanmax(np.abs(got - want) - room), np.argwhere(bad)[0])
+    return got
+
+
+ATTENTION_CASES = [
+    # nbat, ntimes, nhead, nkv, npiece, page, lens, counts, tree
+    (1, 1, 1, 1, 16, 4, [0], None, False),                       # its own key alone
+    (1, 1, 2, 1, 16, 4, [1], None, False),
+    (3, 1, 4, 2, 64, 16, [40, 0, 77], None, False),              # decode
+    (2, 1, 32, 8, 128, 64, [700, 1023], None, False),
+    (2, 5, 4, 4, 64, 7, [33, 12], [5, 2], False),                # a run of tokens, pages that end inside a tile
+    (2, 17, 6, 2, 32, 48, [100, 63], [17, 11], True),
+    (2, 33, 2, 1, 128, 50, [64, 31], None, True),                # more than one mask word
+    (1, 70, 8, 2, 64, 32, [130], None, True),
+    (1, 70, 3, 3, 80, 32, [0], None, True),
+    (2, 9, 8, 1, 96, 16, [300, 5], [9, 0], True),                # a sequence without new tokens
+    (1, 16, 8, 2, 128, 256, [3000], None, True),                 # several parts
+    (1, 3, 2, 2, 256, 16, [90], None, False),
+    (1, 130, 4, 1, 64, 64, [500], None, False),                  # many rows a key head
+    (2, 4, 3, 1, 20, 5, [33, 14], None, True),                   # heads off 16 elements
+    (2, 4, 3, 3, 7, 5, [33, 14], None, True),
+    (4, 2, 4, 2, 64, 16, [-5, 0, 3, 30], [2, 9, -1, 1], False),  # lengths and counts out of range
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(ATTENTION_CASES)))
+def test_cache_attention(case):
+    rng = np.random.default_rng(100 + case)
+    c = _attention_case(rng, *ATTENTION_CASES[case])
+    got = _check_attention(c)
+    assert np.array_equal(got, _attend(c)), "the same call twice gives the same bits"
+
+
+@pytest.mark.gpu
+def test_cache_attention_strides_and_alignment():
+    rng = np.random.default_rng(7)
+    c = _attention_case(rng, 2, 6, 4, 2, 64, 16, [50, 21], [6, 3], True, extra=17)
+    _check_attention(c)
+    _check_attention(c, q_off=1)
+    _check_attention(c, c_off=1)
+    _check_attention(c, q_off=3, c_off=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("npiece", [64, 20])
+def test_cache_attention_rows_that_see_nothing(npiece):
+    rng = np.random.default_rng(8)
+    c = _attention_case(rng, 2, 8, 4, 2, npiece, 16, [0, 40], None, True)
+    c["see_new"][0, 3] = False
+    c["see_new"][0, 0] = False
+    got = _check_attention(c)
+    assert np.all(got[0, 3] == 0) and np.all(got[0, 0] == 0)
+    # pages that do not exist: all of one sequence, one in the middle of the other
+    c["table"][0, :] = -1
+    c["table"][1, 1] = c["npage"]
+    got = _check_attention(c)
+    assert np.all(got[0] == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("npiece", [64, 128, 20])
+@pytest.mark.parametrize("poison", [np.nan, np.inf, -np.inf])
+def test_cache_attention_keys_that_are_not_seen_do_not_matter(npiece, poison):
+    rng = np.random.default_rng(9)
+    c = _attention_case(rng, 2, 11, 4, 2, npiece, 16, [37, 5], [11, 6], True)
+    c["see_new"][:, :, 4] = False               # new token 4 is seen by nobody, token 2 by some
+    clean = _attend(c)
+    want, room = _expected(c)
+    for b, (n, count) in enumerate(zip(c["lens"], c["counts"])):
+        for at in [n + 4] + list(range(n + count, c["page"] * c["most"])):   # and what stands behind the sequence
+            for name in ("ck", "cv"):
+                c[name][c["table"][b, at // 16], at % 16] = poison
+    rest = sorted(set(range(c["npage"])) - set(c["table"].ravel()))
+    c["ck"][rest], c["cv"][rest] = poison, poison
+    assert np.array_equal(_attend(c), clean)
+    # a key that some rows see: the others are as before
+    n = c["lens"][0]
+    for name in ("ck", "cv"):
+        c[name][c["table"][0, (n + 2) // 16], (n + 2) % 16] = poison
+    got = _attend(c)
+    hidden = ~c["see_new"][0][:, 2]
+    assert hidden.any() and not hidden.all()
+    assert np.all(np.abs(got[0][hidden] - want[0][hidden]) <= room[0][hidden])
+    assert np.array_equal(got[1], clean[1])
+
+
+@pytest.mark.gpu
+def test_cache_attention_large_and_equal_scores():
+    rng = np.random.default_rng(10)
+    c = _attention_case(rng, 1, 4, 2, 1, 64, 16, [200], None, False, scale=40.0)
+    _check_attention(c)                          # scores of hundreds: one key holds nearly all the weight
+    c["q"][:] = 0.0
+    _check_attention(c)                          # all scores equal
+    _check_attention(c, coef=0.0)
+    c = _attention_case(rng, 1, 4, 2, 1, 64, 16, [200], None, False)
+    c["ck"] *= 1e-30
+    _check_attention(c)
+
+
+@pytest.mark.gpu
+def test_cache_attention_one_page_a_sequence_without_a_table():
+    rng = np.random.default_rng(11)
+    c = _attention_case(rng, 3, 2, 4, 2, 64, 128, [100, 3, 60], None, False)
+    c["table"] = np.arange(3, dtype=np.int32).reshape(3, 1)
+    want, room = _expected(c)
+    y = Tensor((3, 2, 256))
+    q, ck, cv = (DeviceBuffer.from_numpy(c[n]) for n in ("q", "ck", "cv"))
+    VMath.cache_attention(0, y.ptr, q, ck, cv, None, dev_int(c["lens"]), None, None, 3, 2, 256, 4, 2, 64, c["npage"], 128, 1,
+                          kai.hyper(0.125))
+    assert np.all(np.abs(y.numpy().reshape(want.shape) - want) <= room)
+
+
+# ---- the gated projection -----------------------------------------------------------------------------------------
+
+GATED_SIZES = [(1, 64, 64), (1, 4096, 96), (2, 100, 33), (5, 777, 130), (16, 256, 512), (17, 96, 48), (24, 1024, 320),
+               (33, 512, 64), (64, 784, 512), (65, 65, 65), (100, 1, 7), (3, 5, 1), (130, 200, 258), (256, 1024, 300),
+               (300, 301, 259), (513, 128, 640)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat,xvec,yvec", GATED_SIZES)
+@pytest.mark.parametrize("bias", [False, True])
+def test_gated_forward_and_backward(ndat, xvec, yvec, bias):
+    rng = np.random.default_rng(ndat + xvec + yvec)
+    name = list(ACTS)[(ndat + yvec) % len(ACTS)]
+    act, slope = ACTS[name]
+    x = rng.standard_normal((ndat, xvec)).astype(np.float32)
+    wg, wu = ((rng.uniform(-1, 1, (yvec, xvec)) * xvec ** -0.5).astype(np.float32) for _ in range(2))
+    bg, bu = (rng.standard_normal(yvec).astype(np.float32) for _ in range(2)) if bias else (None, None)
+    gy = rng.standard_normal((ndat, yvec)).astype(np.float32)
+    f8 = lambda a: None if a is None else a.astype(np.float64)
+    gate, up = f8(x) @ f8(wg).T, f8(x) @ f8(wu).T
+    if bias:
+        gate, up = gate + bg, up + bu
+    T = lambda a: None if a is None else Tensor.from_numpy(a)
+    tx, twg, twu, tbg, tbu, tgy = (T(a) for a in (x, wg, wu, bg, bu, gy))
+    y = gated(tx, twg, twu, tbg, tbu, actfunc=name, leaky_alpha=0.25, keep=True)
+    assert rel_fro(y.numpy(), act(gate) * up) <= REL_FRO_TOL
+    assert rel_fro(y.saved["gate"].numpy(), gate) <= REL_FRO_TOL
+    assert rel_fro(y.saved["up"].numpy(), up) <= REL_FRO_TOL
+    short = gated(tx, twg, twu, tbg, tbu, actfunc=name, leaky_alpha=0.25)
+    assert np.array_equal(short.numpy(), y.numpy()), "without the kept sums the same result"
+    # the gradients from exactly the sums that the call is given
+    g32, u32 = f8(y.saved["gate"].numpy()), f8(y.saved["up"].numpy())
+    gg, gu = gy * u32 * slope(g32), gy * act(g32)
+    got = gated_backprop(y, tgy)
+    want = {"x": gg @ f8(wg) + gu @ f8(wu), "wg": gg.T @ f8(x), "wu": gu.T @ f8(x), "bg": gg.sum(0), "bu": gu.sum(0)}
+    for k, g in got.items():
+        assert rel_fro(g.numpy(), want[k]) <= REL_FRO_TOL, k
+    assert set(got) == ({"x", "wg", "wu", "bg", "bu"} if bias else {"x", "wg", "wu"})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", list(ACTS))
+def test_gated_gradient_against_differences(act):
+    rng = np.random.default_rng(21)
+    ndat, xvec, yvec = 9, 12, 10
+    f, slope = ACTS[act]
+    shapes = {"x": (ndat, xvec), "wg": (yvec, xvec), "wu": (yvec, xvec), "bg": (yvec,), "bu": (yvec,)}
+    v = {k: rng.standard_normal(s).astype(np.float32) for k, s in shapes.items()}
+    gy = rng.standard_normal((ndat, yvec)).astype(np.float32)
+    value = lambda d: np.sum(f(d["x"] @ d["wg"].T + d["bg"]) * (d["x"] @ d["wu"].T + d["bu"]) * gy)
+    t = {k: Tensor.from_numpy(a) for k, a in v.items()}
+    y = gated(t["x"], t["wg"], t["wu"], t["bg"], t["bu"], actfunc=act, leaky_alpha=0.25, keep=True)
+    got = gated_backprop(y, Tensor.from_numpy(gy))
+    v = {k: a.astype(np.float64) for k, a in v.items()}
+    h = 1e-5
+    for name, s in shapes.items():
+        for _ in range(6):
+            e = np.zeros(s)
+            e[tuple(rng.integers(0, n) for n in s)] = h
+            diff = (value(dict(v, **{name: v[name] + e})) - value(dict(v, **{name: v[name] - e}))) / (2 * h)
+            at = np.sum(got[name].numpy() * (e / h))
+            # differences in 64 bits are off by about h^2 and 2^-53 / h, both below 1e-9 of sums of a hundred terms
+            assert abs(at - diff) <= 1e-5 * (1 + np.abs(got[name].numpy()).max()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat", [1, 20, 70])
+def test_gated_accumulates_and_leaves_out(ndat):
+    rng = np.random.default_rng(22)
+    xvec, yvec = 72, 40
+    act, slope = ACTS["swish"]
+    r = lambda *s: rng.standard_normal(s).astype(np.float32)
+    x, wg, wu, gate, up, gy = r(ndat, xvec), r(yvec, xvec), r(yvec, xvec), r(ndat, yvec), r(ndat, yvec), r(ndat, yvec)
+    g8, u8 = gate.astype(np.float64), up.astype(np.float64)
+    gg, gu = gy * u8 * slope(g8), gy * act(g8)
+    want = {"gx": gg @ wg + gu @ wu, "gwg": gg.T @ x, "gwu": gu.T @ x, "gbg": gg.sum(0), "gbu": gu.sum(0)}
+    put = DeviceBuffer.from_numpy
+    b = {n: put(a) for n, a in (("x", x), ("wg", wg), ("wu", wu), ("gate", gate), ("up", up), ("gy", gy))}
+    names = ["gx", "gwg", "gwu", "gbg", "gbu"]
+    for missing in [None] + names:
+        for work in (None, put(np.zeros(2 * ndat * yvec, np.float32))):
+            old = {n: r(*want[n].shape) for n in names}
+            out = {n: None if n == missing else put(old[n]) for n in names}
+            VMath.gated_backward(0, out["gx"], out["gwg"], out["gwu"], out["gbg"], out["gbu"], work, b["gy"], b["wg"], b["wu"],
+                                 b["x"], b["gate"], b["up"], yvec, ndat, xvec, ACT["swish"], None, True)
+            for n in names:
+                if n != missing:
+                    assert rel_fro(out[n].to_numpy(want[n].shape), want[n] + old[n]) <= REL_FRO_TOL, (n, missing)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat,yvec", [(1, 40), (20, 40), (200, 300)])
+def test_gated_alignment_and_bounds(ndat, yvec):
+    """Buffers 4 bytes off 16-byte lines give what aligned ones give, and nothing is written beside the outputs."""
+    rng = np.random.default_rng(23)
+    xvec = 76
+    r = lambda *s: rng.standard_normal(s).astype(np.float32)
+    x, wg, wu, gy = r(ndat, xvec), r(yvec, xvec), r(yvec, xvec), r(ndat, yvec)
+
+    def run(off):
+        put = lambda a: DeviceBuffer.from_numpy(np.concatenate([np.full(off, 3.0, np.float32), a.ravel(), np.full(8, 3.0, np.float32)]))
+        new = lambda *s: (put(np.full(s, 9.0, np.float32)), s)
+        ins = {n: put(a) for n, a in (("x", x), ("wg", wg), ("wu", wu), ("gy", gy))}
+        at = lambda b: b.offset(4 * off)
+        outs = [new(ndat, yvec), new(ndat, yvec), new(ndat, yvec), new(ndat, xvec), new(yvec, xvec), new(yvec, xvec), new(yvec),
+                new(yvec)]
+        y, gate, up, gx, gwg, gwu, gbg, gbu = (at(b) for b, _ in outs)
+        VMath.gated_forward(0, y, gate, up, at(ins["wg"]), at(ins["wu"]), None, None, at(ins["x"]), yvec, ndat, xvec,
+                            ACT["swish"], None)
+        VMath.gated_backward(0, gx, gwg, gwu, gbg, gbu, None, at(ins["gy"]), at(ins["wg"]), at(ins["wu"]), at(ins["x"]), gate, up,
+                             yvec, ndat, xvec, ACT["swish"], None, False)
+        got = []
+        for b, s in outs:
+            n = int(np.prod(s))
+            a = b.to_numpy(off + n + 8)
+            assert np.all(a[:off] == 3.0) and np.all(a[off + n:] == 3.0)
+            got.append(a[off:off + n].reshape(s))
+        return got
+
+    for a, b in zip(run(0), run(1)):
+        assert rel_fro(b, a) <= REL_FRO_TOL
+
+
+@pytest.mark.gpu
+def test_gated_empty_reductions():
+    """No inputs: the biases alone; no rows or no hidden units: gradients of zero, or what was there with acc."""
+    bg, bu = np.array([0.5, -1.0, 2.0], np.float32), np.array([1.0, 2.0, 3.0], np.float32)
+    y = Tensor((4, 3))
+    VMath.gated_forward(0, y.ptr, None, None, None, None, DeviceBuffer.from_numpy(bg), DeviceBuffer.from_numpy(bu), None, 3, 4, 0,
+                        ACT["relu"], None)
+    assert np.array_equal(y.numpy(), np.broadcast_to(np.maximum(bg, 0) * bu, (4, 3)))
+    some = np.full((5, 6), 2.0, np.float32)
+    for acc in (False, True):
+        gx, gw = DeviceBuffer.from_numpy(some), DeviceBuffer.from_numpy(some)
+        VMath.gated_backward(0, gx, None, None, None, None, None, None, None, None, None, None, None, 0, 5, 6, 0, None, acc)
+        VMath.gated_backward(0, None, gw, None, None, None, None, None, None, None, None, None, None, 5, 0, 6, 0, None, acc)
+        for b in (gx, gw):
+            assert np.array_equal(b.to_numpy((5, 6)), some if acc else np.zeros((5, 6), np.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat", [1, 20, 300])
+def test_gated_infinities(ndat):
+    """An infinity or a NaN reaches exactly the sums that it enters, as it does in a plain sum."""
+    rng = np.random.default_rng(24)
+    xvec, yvec = 96, 272
+    x = rng.standard_normal((ndat, xvec)).astype(np.float32)
+    wg, wu = (rng.standard_normal((yvec, xvec)).astype(np.float32) for _ in range(2))
+    x[0, 5], x[0, 2] = np.inf, 0.5
+    wg[7, 9] = np.nan
+    wu[3, 11] = -np.inf
+    wg[4, 2] = 3.402e38
+    wu[6, 1] = 1e-44
+    wg[9] = 0.0
+    with np.errstate(all="ignore"):
+        gate, up = x.astype(np.float64) @ wg.astype(np.float64).T, x.astype(np.float64) @ wu.astype(np.float64).T
+    y = gated(*(Tensor.from_numpy(a) for a in (x, wg, wu)), actfunc="none", keep=True)
+    for got, want in ((y.saved["gate"].numpy(), gate), (y.saved["up"].numpy(), up)):
+        over = np.abs(want) > 3.4028235e38
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[over], np.sign(want[over]) * np.float32(np.inf))
+        fine = ~over & np.isfinite(want)
+        plain = fine.copy()
+        plain[:, 4] = False
+        assert rel_fro(got[plain], want[plain]) <= REL_FRO_TOL
+        assert np.all(np.abs(got[fine] - want[fine]) <= 1e-5 * (np.abs(want[fine]) + 100.0))
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [None, dict(nrot=8), dict(nrot=16, layout="pairs", scaling="linear", factor=2.0)])
+def test_attention_block_with_rotary(rotary):
+    """mh_attention with turned queries and keys: fused and unfused agree with 64 bits, gradients with differences."""
+    rng = np.random.default_rng(31)
+    nbat, ntimes, nhead, npiece = 2, 12, 4, 16
+    nvec = nhead * npiece
+    d = None if rotary is None else kai.rotary_desc(**rotary)
+    x = rng.standard_normal((nbat, ntimes, nvec)).astype(np.float32)
+    w = {n: (rng.standard_normal((nvec, nvec)) / 8).astype(np.float32) for n in ("Kw", "Qw", "Vw", "Ow")}
+    b = {n: rng.standard_normal(nvec).astype(np.float32) for n in ("Kb", "Qb", "Vb", "Ob")}
+    gy = rng.standard_normal(x.shape).astype(np.float32)
+    pos = np.broadcast_to(np.arange(ntimes), (nbat, ntimes))
+
+    def forward(p):
+        out = np.zeros(x.shape)
+        k, q, v = (p["x"] @ p[n + "w"].T + p[n + "b"] for n in "KQV")
+        k, q, v = (a.reshape(nbat, ntimes, nhead, npiece) for a in (k, q, v))
+        if d is not None:
+            k, q = plain_rotary(k, pos, d)[0], plain_rotary(q, pos, d)[0]
+        for i in range(nbat):
+            out[i] = plain_attention(q[i], k[i], v[i], np.tril(np.ones((ntimes, ntimes), bool)), 0.25)[0].reshape(ntimes, nvec)
+        return out @ p["Ow"].T + p["Ob"]
+
+    p = {k: v.astype(np.float64) for k, v in dict(w, **b, x=x).items()}
+    want = forward(p)
+    tx = Tensor.from_numpy(x)
+    args = [Tensor.from_numpy(dict(w, **b)[n]) for n in ("Kw", "Kb", "Qw", "Qb", "Vw", "Vb", "Ow", "Ob")]
+    for fused in (False, True):
+        y = tx.mh_attention(tx, tx, tx, *args, nhead, mask=True, fused=fused, rotary=d)
+        assert rel_fro(y.numpy(), want) <= REL_FRO_TOL
+        g = y.mh_attention_backprop(Tensor.from_numpy(gy), fused=fused)
+        h = 1e-5
+        # the reference's key gradient follows its own row indexing, so only what does not pass through it is held
+        # to differences: the value and the output projections, and the query projection's way through the turn
+        for n in ("Vw", "Ow", "Qw"):
+            e = rng.standard_normal(w[n].shape)
+            diff = np.sum((forward(dict(p, **{n: p[n] + h * e})) - forward(dict(p, **{n: p[n] - h * e}))) * gy) / (2 * h)
+            assert abs(np.sum(g[n].numpy() * e) - diff) <= 1e-4 * np.linalg.norm(g[n].numpy()), n
+
+
+@pytest.mark.gpu
+def test_decoder_steps_equal_the_whole_sequence():
+    """A prompt, single tokens and a drafted tree through projections, cache, attention, gated projection and dense layer:
+    each accepted token's row is what one pass over the whole sequence gives it."""
+    rng = np.random.default_rng(32)
+    nbat, nhead, nkv, npiece, hidden = 2, 4, 2, 32, 96
+    nvec, kvec, prompt, total = nhead * npiece, nkv * npiece, 21, 34
+    d = kai.rotary_desc(32, scaling="parts", factor=4.0, trained=16.0)
+    x = rng.standard_normal((nbat, total, nvec)).astype(np.float32)
+    w = {n: (rng.standard_normal(s) / np.sqrt(s[1])).astype(np.float32) for n, s in (
+        ("q", (nvec, nvec)), ("k", (kvec, nvec)), ("v", (kvec, nvec)), ("o", (nvec, nvec)), ("g", (hidden, nvec)),
+        ("u", (hidden, nvec)), ("d", (nvec, hidden)))}
+    t = {n: Tensor.from_numpy(a) for n, a in w.items()}
+    w8 = {n: a.astype(np.float64) for n, a in w.items()}
+
+    def tail8(mixed):
+        h = mixed @ w8["o"].T
+        return (ACTS["swish"][0](h @ w8["g"].T) * (h @ w8["u"].T)) @ w8["d"].T
+
+    def whole(xs):
+        n = xs.shape[0]
+        pos = np.arange(n)
+        q = plain_rotary((xs @ w8["q"].T).reshape(n, nhead, npiece), pos, d)[0]
+        k = plain_rotary((xs @ w8["k"].T).reshape(n, nkv, npiece), pos, d)[0]
+        v = (xs @ w8["v"].T).reshape(n, nkv, npiece)
+        y, _ = plain_attention(q, k, v, np.tril(np.ones((n, n), bool)), npiece ** -0.5)
+        return tail8(y.reshape(n, nvec))
+
+    want = np.stack([whole(x[b].astype(np.float64)) for b in range(nbat)])
+    cache = KeyValueCache(nbat, nkv, npiece, 8, 8, rotary=d)
+
+    def step(rows, positions, mask=None, counts=None):
+        tx = Tensor.from_numpy(rows)
+        dpos = dev_int(positions)
+        q = rotate(tx.matmul(t["q"]), nhead, d, positions=dpos)
+        cache.append(tx.matmul(t["k"]), tx.matmul(t["v"]), positions=dpos, counts=counts)
+        mixed = cache.attend(q, nhead, mask=mask, counts=counts)
+        return gated(mixed.matmul(t["o"]), t["g"], t["u"]).matmul(t["d"]).numpy()
+
+    got = np.zeros(want.shape, np.float32)
+    run = np.broadcast_to(np.arange(prompt), (nbat, prompt))
+    got[:, :prompt] = step(x[:, :prompt], run)
+    cache.accept(prompt)
+    for n in range(prompt, prompt + 3):
+        got[:, n:n + 1] = step(x[:, n:n + 1], np.full((nbat, 1), n))
+        cache.accept(1)
+    # a draft: the true continuation of five tokens first, then four wrong tokens as side branches
+    n = prompt + 3
+    rows = np.concatenate([x[:, n:n + 5], rng.standard_normal((nbat, 4, nvec)).astype(np.float32)], 1)
+    see = np.zeros((9, 9), bool)
+    see[:5, :5] = np.tril(np.ones((5, 5), bool))
+    depth = [0, 1, 2, 3, 4, 0, 1, 2, 3]
+    for i, parent in ((5, None), (6, 5), (7, 1), (8, 7)):
+        if parent is not None:
+            see[i] = see[parent]
+        see[i, i] = True
+        depth[i] = see[i].sum() - 1
+    words = dev_int(np.broadcast_to(words_of(see), (nbat, 9, 1)))
+    got[:, n:n + 5] = step(rows, n + np.broadcast_to(depth, (nbat, 9)), mask=words)[:, :5]
+    cache.accept(5)
+    n += 5
+    last = step(x[:, n:n + 5], n + np.broadcast_to(np.arange(5), (nbat, 5)), counts=dev_int([5, 2]))
+    got[0, n:n + 5], got[1, n:n + 2] = last[0], last[1, :2]
+    assert np.all(last[1, 2:] == tail8(np.zeros((1, nvec)))), "rows behind the count saw nothing"
+    cache.accept([5, 2])
+    got[1, n + 2:n + 5] = step(x[:, n + 2:n + 5], n + 2 + np.broadcast_to(np.arange(3), (nbat, 3)), counts=dev_int([0, 3]))[1]
+    n += 5
+    assert n == total
+    assert rel_fro(got, want) <= REL_FRO_TOL
