@@ -102,7 +102,7 @@ int cache_pages(const char* who, CachePages* c, const int* ppage, const int* ple
     if (nkvhead < 0 || npage < 0 || npagelen < 0 || nmaxpage < 0)
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": negative dimension");
     if (nkvhead > kMaxWidth || nkvhead * npiece > kMaxWidth || npage > kMaxDim || npagelen > kMaxDim || nmaxpage > kMaxDim ||
-        npagelen * nmaxpage > kMaxDim)
+        npagelen * nmaxpage > kMaxDim || npage * npagelen > kMaxDim)
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": dimension out of range");
     if (ppage == nullptr && (nmaxpage > 1 || npage < nbat))
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": without a page table each sequence has one page, its own");
