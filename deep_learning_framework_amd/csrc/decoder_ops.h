@@ -81,6 +81,22 @@ struct GatedArgs {
     const float* hleaky;
 };
 int launch_gated_forward(const GatedArgs& a, hipStream_t stream);
+
+struct GatedGradArgs {
+    float* gx;              // any of the three may be null
+    float* gwg;
+    float* gwu;
+    const float* ggate;     // gradients of the two sums
+    const float* gup;
+    const float* wg;
+    const float* wu;
+    const float* x;
+    int64_t yvec, ndat, xvec;
+    int acc;
+};
+// gx (+)= ggate . wg + gup . wu, gwg (+)= ggate^T . x, gwu (+)= gup^T . x
+int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream);
+
 // ggate = gy * up * act'(gate), gup = gy * act(gate), n elements each
 int launch_gated_activation_backward(float* ggate, float* gup, const float* gy, const float* gate, const float* up,
                                      int64_t n, int act, const float* hleaky, hipStream_t stream);

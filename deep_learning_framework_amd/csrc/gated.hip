@@ -1,6 +1,7 @@
 // The gated feed-forward projection: y = act(x . wg^T + bg) * (x . wu^T + bu), and its element-wise gradients.
 #include "act_funcs.h"
 #include "decoder_ops.h"
+#include "gated_gemm.h"
 #include "gemm_host.h"
 
 namespace kai {
@@ -47,6 +48,15 @@ int launch_gated_activation_backward(float* ggate, float* gup, const float* gy, 
 }
 
 int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
+    GatedGemm p{};
+    p.A[0] = a.x; p.B[0] = a.wg; p.B[1] = a.wu;
+    p.C[0] = a.y; p.C[1] = a.gate; p.C[2] = a.up;
+    p.bias[0] = a.bg; p.bias[1] = a.bu;
+    p.hleaky = a.hleaky; p.act = a.act;
+    p.M = a.ndat; p.N = a.yvec; p.K = (int)a.xvec;
+    p.lda = p.ldb = a.xvec; p.ldc = a.yvec;
+    p.nwhich = 1;
+    if (a.ndat > 32 && gated_gemm_applies(p)) return launch_gated_gemm(kGatedForward, p, stream);
     // both products, then the activation and the product; the pre-activations in the caller's buffers or in scratch
     const int64_t n = a.ndat * a.yvec;
     float* gate = a.gate;
@@ -66,6 +76,43 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
         KAI_TRY(launch_gemm(d, stream));
     }
     return launch_gated_activation(a.y, gate, up, n, a.act, a.hleaky, stream);
+}
+
+int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
+    GatedGemm p{};
+    p.A[0] = a.ggate; p.A[1] = a.gup;
+    p.acc = a.acc;
+    p.nwhich = 1;
+    if (a.gx) {
+        p.B[0] = a.wg; p.B[1] = a.wu;
+        p.C[0] = a.gx;
+        p.M = a.ndat; p.N = a.xvec; p.K = (int)a.yvec;
+        p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
+        if (a.ndat > 32 && gated_gemm_applies(p)) {
+            KAI_TRY(launch_gated_gemm(kGatedGx, p, stream));
+        } else {
+            KAI_TRY(kai_matmul_backward_x(0, a.gx, a.ggate, a.wg, a.yvec, a.ndat, a.xvec, a.acc));
+            KAI_TRY(kai_matmul_backward_x(0, a.gx, a.gup, a.wu, a.yvec, a.ndat, a.xvec, 1));
+        }
+    }
+    if (a.gwg == nullptr && a.gwu == nullptr) return KAI_OK;
+    p.B[0] = a.x; p.B[1] = nullptr;
+    p.M = a.yvec; p.N = a.xvec; p.K = (int)a.ndat;
+    p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
+    if (a.ndat > 32 && gated_gemm_applies(p)) {
+        p.C[0] = a.gwg; p.C[1] = a.gwu;
+        p.nwhich = 2;
+        if (a.gwg == nullptr || a.gwu == nullptr) {
+            p.nwhich = 1;
+            p.C[0] = a.gwg ? a.gwg : a.gwu;
+            p.C[1] = nullptr;
+            p.A[0] = a.gwg ? a.ggate : a.gup;
+        }
+        return launch_gated_gemm(kGatedGw, p, stream);
+    }
+    if (a.gwg) KAI_TRY(kai_matmul_backward_w(0, a.gwg, a.ggate, a.x, a.yvec, a.ndat, a.xvec, a.acc));
+    if (a.gwu) KAI_TRY(kai_matmul_backward_w(0, a.gwu, a.gup, a.x, a.yvec, a.ndat, a.xvec, a.acc));
+    return KAI_OK;
 }
 
 }  // namespace kai

@@ -207,14 +207,13 @@ int kai_gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* 
     }
     ScratchHold held(held_bytes);
     if (pgbg) KAI_TRY(kai_add_bias_backward_b(device, pgbg, work, ndat, yvec, acc));
-    if (pgbu) KAI_TRY(kai_add_bias_backward_b(device, pgbu, work + n, ndat, yvec, acc));
-    if (pgx) {
-        KAI_TRY(kai_matmul_backward_x(device, pgx, work, pwg, yvec, ndat, xvec, acc));
-        KAI_TRY(kai_matmul_backward_x(device, pgx, work + n, pwu, yvec, ndat, xvec, 1));
-    }
-    if (pgwg) KAI_TRY(kai_matmul_backward_w(device, pgwg, work, px, yvec, ndat, xvec, acc));
-    if (pgwu) KAI_TRY(kai_matmul_backward_w(device, pgwu, work + n, px, yvec, ndat, xvec, acc));
-    return KAI_OK;
+    if (pgbu) KAI_TRY(kai_add_bias_backward_b(device, pgbu, n > 0 ? work + n : nullptr, ndat, yvec, acc));
+    GatedGradArgs a{};
+    a.gx = pgx; a.gwg = pgwg; a.gwu = pgwu;
+    a.ggate = work; a.gup = n > 0 ? work + n : nullptr;
+    a.wg = pwg; a.wu = pwu; a.x = px;
+    a.yvec = yvec; a.ndat = ndat; a.xvec = xvec; a.acc = acc != 0;
+    return launch_gated_gradients(a, current_stream());
 }
 
 }  // extern "C"
