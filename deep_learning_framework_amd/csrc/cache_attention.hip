@@ -6,6 +6,8 @@
 // 32 bits; a row that sees nothing gives zeros.  Few rows meet many keys, so the keys of a sequence are cut into
 // parts that run as separate workgroups; cache_attention_join_kernel adds the parts,
 //   y = sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s.
+#include <type_traits>
+
 #include "decoder_ops.h"
 #include "split_bf16.h"
 
@@ -16,6 +18,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWave = 64;
 constexpr int kMaxPiece = 256;
+constexpr int kMaxParts = 256;   // a thread of the joining workgroup each
 constexpr int kKeyStep = 32;     // a part of a sequence's keys is a whole number of these
 
 struct Parts {
@@ -60,6 +63,26 @@ __device__ bool sees_new(const int* mask, int64_t ntimes, int64_t b, int t, int 
     if (mask == nullptr) return s <= t;
     const int64_t nword = (ntimes + 31) / 32;
     return ((unsigned)mask[(b * ntimes + t) * nword + s / 32] >> (s & 31)) & 1u;
+}
+
+// Which of the keys j .. j + 7 new token t sees, as bits; none for rows behind the count.  Keys behind the new ones are the
+// caller's to leave out.
+__device__ __forceinline__ unsigned eight_seen(const int* mask, int64_t ntimes, const Sequence& seq, int64_t b, int t, int j) {
+    if (t >= seq.count) return 0u;
+    const int s = j - seq.len;
+    if (s <= -8) return 0xFFu;
+    const int from = s < 0 ? 0 : s;
+    unsigned bits;
+    if (mask == nullptr) {
+        const int seen = t + 1 - from;       // new tokens from `from` on
+        bits = seen >= 8 ? 0xFFu : seen <= 0 ? 0u : (1u << seen) - 1;
+    } else {
+        const int nword = (int)((ntimes + 31) / 32), w = from / 32 < nword ? from / 32 : nword - 1;
+        const unsigned* words = reinterpret_cast<const unsigned*>(mask) + (b * ntimes + t) * nword;
+        const unsigned lo = words[w], hi = words[w + 1 < nword ? w + 1 : w];
+        bits = (unsigned)((((uint64_t)hi << 32) | lo) >> (from & 31)) & 0xFFu;
+    }
+    return s < 0 ? (bits << -s | ((1u << -s) - 1)) & 0xFFu : bits;
 }
 
 // Results of a row: straight to y, or the part's sums.
@@ -153,11 +176,22 @@ template <int VW, int NR>
 struct Tiled {
     static constexpr int np = 16 * VW;
     static constexpr int KC = (np + 31) / 32;
-    static constexpr int kRegs = NR * (4 * VW + 2);                                  // of a wave's result, per lane
-    static constexpr int kQueryBytes = 3 * KC * NR * kWave * 16;
-    static constexpr int kMergeBytes = 2 * kRegs * kWave * 4;
-    static constexpr int kLds = (kQueryBytes > kMergeBytes ? kQueryBytes : kMergeBytes) + 16;
+    static constexpr int kQueryChunks = KC * NR * kWave;                 // of 8 elements, and three planes of them
+    static constexpr int kQueryBytes = 3 * kQueryChunks * 16;
+    static constexpr int kWaveChunks = NR * VW * kWave;                  // of a wave's result, 4 elements each
+    static constexpr int kMergeBytes = 4 * kWaveChunks * 16;
+    static constexpr int kRows = 16 * NR;
+    static constexpr int kLds = (kQueryBytes > kMergeBytes ? kQueryBytes : kMergeBytes);
 };
+
+// f(0), ..., f(N - 1) with compile-time indices
+template <int B, int E, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (B < E) {
+        f(std::integral_constant<int, B>{});
+        static_for<B + 1, E>(f);
+    }
+}
 
 template <int N>
 __device__ __forceinline__ void load_floats(float* to, const float* from) {
@@ -178,20 +212,38 @@ __device__ __forceinline__ void load_floats(float* to, const float* from) {
     if constexpr (N % 2 == 1) to[N - 1] = from[N - 1];
 }
 
-__device__ __forceinline__ f32x4 mfma6(const Split8& a, const Split8& b, f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.h, b.l, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.l, b.h, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.m, b.m, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.h, b.m, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.m, b.h, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.h, b.h, c, 0, 0, 0);
+// c[i] += a(i) . b(i), the small products first, a product's turn going round the N independent sums
+template <int N, typename A, typename B>
+__device__ __forceinline__ void mfma6(f32x4* const* c, A&& a, B&& b) {
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).h, b(i).l, *c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).l, b(i).h, *c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).m, b(i).m, *c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).h, b(i).m, *c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).m, b(i).h, *c[i], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) *c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(i).h, b(i).h, *c[i], 0, 0, 0);
+}
+
+// Asks the scheduler to spread the N matrix instructions of a block of code over its vector instructions.
+template <int N>
+__device__ __forceinline__ void interleave() {
+    static_for<0, N>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+    });
 }
 
 template <int VW, int NR>
-__global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_tiled_kernel(CacheAttentionArgs a, Parts parts, int row_tiles) {
+__global__ __launch_bounds__(256, VW * NR > 16 ? 1 : 2) void cache_attention_tiled_kernel(CacheAttentionArgs a, Parts parts, int row_tiles) {
     using T = Tiled<VW, NR>;
     constexpr int np = T::np, KC = T::KC;
     extern __shared__ char lds[];
+    __shared__ float2 part_ml[4][T::kRows];
     const CachePages& c = a.pages;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int n = lane & 15, g = lane >> 4;
@@ -200,8 +252,22 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
     const int bh = (int)(blockIdx.x / (unsigned)row_tiles);
     const int kvh = bh % c.nkvhead, b = bh / c.nkvhead;
     const int group = a.nhead / c.nkvhead;
+    const int row0 = tile * T::kRows;
+    // The start is one chain of loads: lengths, page, keys.  The queries come meanwhile.
+    constexpr int kQueryLoads = (T::kQueryChunks + 256 - 1) / 256;
+    float qx[kQueryLoads][8];
+#pragma unroll
+    for (int i = 0; i < kQueryLoads; i++) {
+        const int e = (int)threadIdx.x + 256 * i;
+        const int row = row0 + 16 * (e / kWave % NR) + (e & 15), d = 32 * (e / (kWave * NR)) + (e >> 4 & 3) * 8;
+        const int t = row / group, h = kvh * group + (row - t * group);
+#pragma unroll
+        for (int k = 0; k < 8; k++) qx[i][k] = 0.0f;
+        if (e < T::kQueryChunks && t < c.ntimes && d < np)
+            load_floats<8>(qx[i], a.q + ((int64_t)b * c.ntimes + t) * a.ldq + (int64_t)h * np + d);
+    }
     const Sequence seq = sequence_of(c, b);
-    const int nrow = seq.count * group, row0 = tile * 16 * NR;
+    const int nrow = seq.count * group;
     if (row0 >= nrow) return;
     int begin, end;
     part_of(seq.keys, parts.nsplit, split, &begin, &end);
@@ -209,51 +275,44 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
     const float* ck = a.ck + (int64_t)kvh * np;
     const float* cv = a.cv + (int64_t)kvh * np;
 
-    // the queries, times coef, as three planes of right operands: chunk (plane, kk, r) holds lane's 8 elements
-    bf16x8* query = reinterpret_cast<bf16x8*>(lds);
-    {
-        const float coef = a.hcoef ? *a.hcoef : 0.0f;
-        for (int e = threadIdx.x; e < KC * NR * kWave; e += 256) {
-            const int el = e & (kWave - 1), r = e / kWave % NR, kk = e / (kWave * NR);
-            const int row = row0 + 16 * r + (el & 15), d = 32 * kk + 8 * (el >> 4);
-            float x[8] = {};
-            if (row < nrow && d < np) {
-                const int t = row / group, h = kvh * group + (row - t * group);
-                load_floats<8>(x, a.q + ((int64_t)b * c.ntimes + t) * a.ldq + (int64_t)h * np + d);
-            }
-            const Split8 s = split8([&](int i) { return x[i] * coef; });
-            query[e] = s.h;
-            query[e + KC * NR * kWave] = s.m;
-            query[e + 2 * KC * NR * kWave] = s.l;
-        }
-    }
-    __syncthreads();
-    const auto query_at = [&](int kk, int r) {
-        const int e = (kk * NR + r) * kWave + lane;
-        return Split8{query[e], query[e + KC * NR * kWave], query[e + 2 * KC * NR * kWave]};
-    };
-
     // rows of the cache of a tile's 32 keys, in lanes 0..31 (and once more in 32..63); -1: no such key
     const auto rows_of = [&](int j0) {
         const int j = j0 + (lane & 31);
         return j < end ? (int)row_of_key(c, b, j) : -1;
     };
-    float kf[2][KC][8];
-    const auto load_keys = [&](int rows) {
+    // Where a key does not exist row 0 is loaded and not used.
+    const auto existing = [](int row) { return (int64_t)(row < 0 ? 0 : row); };
+    float kf[2][KC][8], vf[8][VW];
+    unsigned there = 0;
+    const auto load_key = [&](const float* key, int kb, int kk) {
+        if (np % 32 == 0 || kk < KC - 1 || g < 2) {
+            load_floats<8>(kf[kb][kk], key + 32 * kk);
+        } else {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            const int row = __shfl(rows, 8 * (n >> 2) + 4 * kb + (n & 3));
-            const float* from = ck + (int64_t)(row < 0 ? 0 : row) * width + 8 * g;
-#pragma unroll
-            for (int kk = 0; kk < KC; kk++) {
-                if (np % 32 == 0 || kk < KC - 1 || g < 2) {
-                    load_floats<8>(kf[kb][kk], from + 32 * kk);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) kf[kb][kk][i] = 0.0f;
-                }
-            }
+            for (int i = 0; i < 8; i++) kf[kb][kk][i] = 0.0f;
         }
+    };
+    const auto key_of = [&](int rows, int kb) {
+        return ck + existing(__shfl(rows, 8 * (n >> 2) + 4 * kb + (n & 3))) * width + 8 * g;
+    };
+    int vrow[8];
+    const auto value_rows = [&](int rows) {
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            vrow[i] = __shfl(rows, 8 * g + i);
+            there |= vrow[i] < 0 ? 0u : 1u << i;
+        }
+    };
+    constexpr int kGroups = (VW + 3) / 4;
+    // With one tile of rows a wave, each register is loaded for the wave's next tile as soon as this tile's use of it is
+    // over.  With more rows there is no room for a whole tile in flight (two waves of a SIMD share its 512 registers): the
+    // values' second half and the next keys' two halves follow one another through the same registers.
+    constexpr bool kLate = NR == 2 && VW > 4;
+    const auto load_values = [&](auto group) {
+        constexpr int j0 = 4 * decltype(group)::value, count = VW - j0 < 4 ? VW - j0 : 4;
+#pragma unroll
+        for (int i = 0; i < 8; i++) load_floats<count>(vf[i] + j0, cv + existing(vrow[i]) * width + VW * n + j0);
     };
 
     f32x4 o[NR][VW];
@@ -265,39 +324,73 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
 #pragma unroll
         for (int j = 0; j < VW; j++) o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    int rows = rows_of(begin + 32 * wave);
-    if (begin + 32 * wave < end) load_keys(rows);
-    for (int j0 = begin + 32 * wave; j0 < end; j0 += 128) {
+    const int first = begin + 32 * wave;
+    if (first < end) {
+        const int rows = rows_of(first);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int kk = 0; kk < KC; kk++) load_key(key_of(rows, kb), kb, kk);
+        value_rows(rows);
+        if constexpr (!kLate) static_for<0, kGroups>(load_values);
+    }
+    // the queries, times coef, as three planes of right operands: chunk (plane, kk, r) holds a lane's 8 elements
+    bf16x8* query = reinterpret_cast<bf16x8*>(lds);
+    {
+        const float coef = a.hcoef ? *a.hcoef : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kQueryLoads; i++) {
+            const int e = (int)threadIdx.x + 256 * i;
+            if (e >= T::kQueryChunks) break;
+            const Split8 s = split8([&](int k) { return qx[i][k] * coef; });
+            query[e] = s.h;
+            query[e + T::kQueryChunks] = s.m;
+            query[e + 2 * T::kQueryChunks] = s.l;
+        }
+    }
+    __syncthreads();
+    const auto query_at = [&](int kk, int r) {
+        const int e = (kk * NR + r) * kWave + lane;
+        return Split8{query[e], query[e + T::kQueryChunks], query[e + 2 * T::kQueryChunks]};
+    };
+    int next_rows = rows_of(first + 128);
+    for (int j0 = first; j0 < end; j0 += 128) {
         // the queries are read from LDS anew for each tile: kept in registers they would crowd out loads in flight
         __asm__ volatile("" ::: "memory");
-        // values of the lane's eight keys
-        float vf[8][VW];
-        unsigned there = 0;
+        const bool masked = j0 + 32 > seq.len || __any(there != 0xFFu);     // in most tiles every row sees every key
+        unsigned sees[NR], seen_by_some = 0;
+        if (masked) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int row = __shfl(rows, 8 * g + i);
-            there |= row < 0 ? 0u : 1u << i;
-            load_floats<VW>(vf[i], cv + (int64_t)(row < 0 ? 0 : row) * width + VW * n);
+            for (int r = 0; r < NR; r++) sees[r] = there & eight_seen(a.mask, c.ntimes, seq, b, (row0 + 16 * r + n) / group, j0 + 8 * g);
         }
-        // in most tiles every row sees every key
-        const bool masked = j0 + 32 > seq.len || __any(there != 0xFFu);
-        unsigned seen_by_some = 0;
-        const int next_rows = rows_of(j0 + 128);
+        const float* next_key[2] = {key_of(next_rows, 0), key_of(next_rows, 1)};
+        if constexpr (kLate) load_values(std::integral_constant<int, 0>{});
         f32x4 s[NR][2];
 #pragma unroll
         for (int r = 0; r < NR; r++) s[r][0] = s[r][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kk = 0; kk < KC; kk++) {
-            const Split8 k0 = split8([&](int i) { return kf[0][kk][i]; });
-            const Split8 k1 = split8([&](int i) { return kf[1][kk][i]; });
+            const Split8 k[2] = {split8([&](int i) { return kf[0][kk][i]; }), split8([&](int i) { return kf[1][kk][i]; })};
+            if constexpr (!kLate) {
+                load_key(next_key[0], 0, kk);
+                load_key(next_key[1], 1, kk);
+            } else if (kk == (KC - 1) / 2) {
+                static_for<1, kGroups>(load_values);
+            }
+            if constexpr (NR == 1) {
+                const Split8 q = query_at(kk, 0);
+                f32x4* const sums[2] = {&s[0][0], &s[0][1]};
+                mfma6<2>(sums, [&](int i) { return k[i]; }, [&](int) { return q; });
+            } else {
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const Split8 q = query_at(kk, r);
-                s[r][0] = mfma6(k0, q, s[r][0]);
-                s[r][1] = mfma6(k1, q, s[r][1]);
+                for (int r = 0; r < NR; r += 2) {
+                    const Split8 q[2] = {query_at(kk, r), query_at(kk, r + 1)};
+                    f32x4* const sums[4] = {&s[r][0], &s[r][1], &s[r + 1][0], &s[r + 1][1]};
+                    mfma6<4>(sums, [&](int i) { return k[i & 1]; }, [&](int i) { return q[i >> 1]; });
+                }
             }
         }
-        if (j0 + 128 < end) load_keys(next_rows);
+        if constexpr (NR > 1) interleave<12 * KC * NR>();
         Split8 p[NR];
 #pragma unroll
         for (int r = 0; r < NR; r++) {
@@ -305,15 +398,9 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = s[r][i >> 2][i & 3];
             if (masked) {
-                const int row = row0 + 16 * r + n;
-                const int t = row / group;
+                seen_by_some |= sees[r];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int j = j0 + 8 * g + i;
-                    const bool seen = row < nrow && (there >> i & 1u) && (j < seq.len || sees_new(a.mask, c.ntimes, b, t, j - seq.len));
-                    if (seen) seen_by_some |= 1u << i;
-                    else x[i] = -INFINITY;
-                }
+                for (int i = 0; i < 8; i++) x[i] = sees[r] >> i & 1u ? x[i] : -INFINITY;
             }
             float top = x[0];
 #pragma unroll
@@ -332,7 +419,7 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
             const float base = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[i] = exp2f((x[i] - base) * 1.4426950408889634f);
+                x[i] = __builtin_amdgcn_exp2f((x[i] - base) * 1.4426950408889634f);
                 l[r] += x[i];
             }
             p[r] = split8([&](int i) { return x[i]; });
@@ -346,13 +433,30 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
 #pragma unroll
                 for (int j = 0; j < VW; j++) vf[i][j] = seen_by_some >> i & 1u ? vf[i][j] : 0.0f;
         }
+        value_rows(next_rows);
+        if constexpr (!kLate) next_rows = rows_of(j0 + 256);
+        static_for<0, kGroups>([&](auto group) {
+            constexpr int first_j = 4 * decltype(group)::value, last_j = VW < first_j + 4 ? VW : first_j + 4;
 #pragma unroll
-        for (int j = 0; j < VW; j++) {
-            const Split8 v = split8([&](int i) { return vf[i][j]; });
+            for (int j = first_j; j < last_j; j++) {
+                const Split8 v = split8([&](int i) { return vf[i][j]; });
+                f32x4* sums[NR];
 #pragma unroll
-            for (int r = 0; r < NR; r++) o[r][j] = mfma6(v, p[r], o[r][j]);
-        }
-        rows = next_rows;
+                for (int r = 0; r < NR; r++) sums[r] = &o[r][j];
+                mfma6<NR>(sums, [&](int) { return v; }, [&](int i) { return p[i]; });
+            }
+            if constexpr (!kLate) {
+                load_values(group);
+            } else {
+#pragma unroll
+                for (int kk = decltype(group)::value * KC / kGroups; kk < (decltype(group)::value + 1) * KC / kGroups; kk++) {
+                    load_key(next_key[0], 0, kk);
+                    load_key(next_key[1], 1, kk);
+                }
+            }
+        });
+        if constexpr (NR > 1) interleave<6 * VW * NR>();
+        if constexpr (kLate) next_rows = rows_of(j0 + 256);
     }
 #pragma unroll
     for (int r = 0; r < NR; r++) {
@@ -360,121 +464,108 @@ __global__ __launch_bounds__(256, VW * NR <= 12 ? 2 : 1) void cache_attention_ti
         l[r] += __shfl_xor(l[r], 32);
     }
 
-    // the four waves' results: 2 and 3 into 0 and 1, then 1 into 0
-    float* merge = reinterpret_cast<float*>(lds);
+    // The four waves' results meet in LDS.  A thread then takes element i of group g of each sixteenth row's VW blocks: VW
+    // consecutive elements of the row.
+    __syncthreads();
+    f32x4* merge = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-    for (int step = 2; step >= 1; step /= 2) {
-        __syncthreads();
-        if (wave >= step && wave < 2 * step) {
-            float* to = merge + (wave - step) * T::kRegs * kWave + lane;
+    for (int r = 0; r < NR; r++) {
+        if (g == 0) part_ml[wave][16 * r + n] = make_float2(m[r], l[r]);
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                to[(r * (4 * VW + 2)) * kWave] = m[r];
-                to[(r * (4 * VW + 2) + 1) * kWave] = l[r];
-#pragma unroll
-                for (int j = 0; j < VW; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) to[(r * (4 * VW + 2) + 2 + 4 * j + i) * kWave] = o[r][j][i];
-            }
-        }
-        __syncthreads();
-        if (wave < step) {
-            const float* from = merge + wave * T::kRegs * kWave + lane;
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const float om = from[(r * (4 * VW + 2)) * kWave], ol = from[(r * (4 * VW + 2) + 1) * kWave];
-                const float top = fmaxf(m[r], om);
-                const float mine = m[r] == top ? 1.0f : expf(m[r] - top), theirs = om == top ? 1.0f : expf(om - top);
-                m[r] = top;
-                l[r] = l[r] * mine + ol * theirs;
-#pragma unroll
-                for (int j = 0; j < VW; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        o[r][j][i] = o[r][j][i] * mine + from[(r * (4 * VW + 2) + 2 + 4 * j + i) * kWave] * theirs;
-            }
-        }
-    }
-
-    // Infinities and NaN in the cache come out as NaN in any row of the tile, those that do not see them too where others
-    // do: the rows are then done again one by one.
-    int* again = reinterpret_cast<int*>(lds + T::kLds - 16);
-    if (wave == 0) {
-        float test = 0.0f;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            test += l[r] * 0.0f;
-#pragma unroll
-            for (int j = 0; j < VW; j++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) test += o[r][j][i] * 0.0f;
-        }
-        const bool bad = __any(test != 0.0f);
-        if (lane == 0) *again = bad;
-        if (!bad) {
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const int row = row0 + 16 * r + n;
-                if (row < nrow) {
-                    const int t = row / group, h = kvh * group + (row - t * group);
-                    const int64_t at = ((int64_t)b * c.ntimes + t) * a.nhead + h;
-                    float* out = a.y + at * np;
-                    float inv = 1.0f;
-                    if (parts.nsplit > 1) {
-                        const int64_t slot = slot_of(parts, c.nbat * c.ntimes * a.nhead, at, split);
-                        if (g == 0) parts.ml[slot] = make_float2(m[r], l[r]);
-                        out = parts.acc + slot * np;
-                    } else {
-                        inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int j = 0; j < VW; j++) out[(4 * g + i) * VW + j] = o[r][j][i] * inv;
-                }
-            }
-        }
+        for (int j = 0; j < VW; j++) merge[((wave * NR + r) * VW + j) * kWave + lane] = o[r][j];
     }
     __syncthreads();
-    if (*again) {
-        for (int row = row0 + wave; row < nrow && row < row0 + 16 * NR; row += 4) {
+    // Infinities and NaN in the cache come out as NaN in any row of the tile, those that do not see them too where others
+    // do: the rows are then done again one by one.
+    float test = 0.0f;
+    const int i = threadIdx.x & 3, rn = threadIdx.x >> 2 & 15, rg = wave;
+#pragma unroll 1
+    for (int r = 0; r < NR; r++) {
+        const int row = row0 + 16 * r + rn;
+        if (row >= nrow) break;
+        float2 ml[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) ml[w] = part_ml[w][16 * r + rn];
+        const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+        float sum = 0.0f, v[VW] = {};
+        const float* from = reinterpret_cast<const float*>(merge + r * VW * kWave + rg * 16 + rn) + i;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float scale = ml[w].x == top ? 1.0f : expf(ml[w].x - top);
+            sum += ml[w].y * scale;
+#pragma unroll
+            for (int j = 0; j < VW; j++) v[j] += from[(w * T::kWaveChunks + j * kWave) * 4] * scale;
+        }
+        const int t = row / group, h = kvh * group + (row - t * group);
+        const int64_t at = ((int64_t)b * c.ntimes + t) * a.nhead + h;
+        float* out = a.y + at * np;
+        float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (parts.nsplit > 1) {
+            const int64_t slot = slot_of(parts, c.nbat * c.ntimes * a.nhead, at, split);
+            if (threadIdx.x % 4 == 0 && rg == 0) parts.ml[slot] = make_float2(top, sum);
+            out = parts.acc + slot * np;
+            inv = 1.0f;
+        }
+        test += sum * 0.0f;
+#pragma unroll
+        for (int j = 0; j < VW; j++) {
+            test += v[j] * 0.0f;
+            out[(4 * rg + i) * VW + j] = v[j] * inv;
+        }
+    }
+    if (__syncthreads_or(test != 0.0f)) {
+#pragma unroll 1
+        for (int row = row0 + wave; row < nrow && row < row0 + T::kRows; row += 4) {
             const int t = row / group;
             attend_row(a, parts, seq, b, t, kvh * group + (row - t * group), split, begin, end);
         }
     }
 }
 
-// A wave for a row: y = sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s over the parts that saw a key.
+// A workgroup for a row: y = sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s over the parts that saw a key.  Each thread
+// finds a part's weight; then the four waves take every fourth part, the lanes along the head, and meet in LDS.
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentionArgs a, Parts parts) {
-    const int lane = threadIdx.x & (kWave - 1);
+    __shared__ float weight[kMaxParts], scratch[8], sums[4][kMaxPiece];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const CachePages& c = a.pages;
-    const int64_t rows = c.nbat * c.ntimes * a.nhead;
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    if (row >= rows) return;
+    const int64_t rows = c.nbat * c.ntimes * a.nhead, row = blockIdx.x;
     const int64_t bt = row / a.nhead;
     const Sequence seq = sequence_of(c, (int)(bt / c.ntimes));
     if ((int)(bt % c.ntimes) >= seq.count) return;
-    float top = -INFINITY;
-    for (int s = 0; s < parts.nsplit; s++) top = fmaxf(top, parts.ml[(int64_t)s * rows + row].x);
-    float sum = 0.0f;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if ((int)threadIdx.x < parts.nsplit) ml = parts.ml[slot_of(parts, rows, row, threadIdx.x)];
+    float top = ml.x;
+#pragma unroll
+    for (int w = 1; w < kWave; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+    if (lane == 0) scratch[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
+    // a part that saw no key has a sum of 0
+    const float mine = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : expf(ml.x - top);
+    weight[threadIdx.x] = mine;
+    float sum = mine == 0.0f ? 0.0f : mine * ml.y;
+#pragma unroll
+    for (int w = 1; w < kWave; w *= 2) sum += __shfl_xor(sum, w);
+    if (lane == 0) scratch[4 + wave] = sum;
+    __syncthreads();
+    sum = scratch[4] + scratch[5] + scratch[6] + scratch[7];
     float acc[kMaxPiece / kWave] = {};
-    for (int s = 0; s < parts.nsplit; s++) {
-        const int64_t slot = (int64_t)s * rows + row;
-        const float2 ml = parts.ml[slot];
-        if (ml.y == 0.0f) continue;
-        const float w = ml.x == top ? 1.0f : expf(ml.x - top);
-        sum += w * ml.y;
+#pragma unroll 4
+    for (int s = wave; s < parts.nsplit; s += 4) {
+        const float w = weight[s];
+        const float* from = parts.acc + slot_of(parts, rows, row, s) * c.npiece;
 #pragma unroll
         for (int i = 0; i < kMaxPiece / kWave; i++) {
             const int d = lane + i * kWave;
-            if (d < c.npiece) acc[i] += w * parts.acc[slot * c.npiece + d];
+            const float v = d < c.npiece ? from[d] : 0.0f;
+            if (w != 0.0f) acc[i] += w * v;
         }
     }
 #pragma unroll
-    for (int i = 0; i < kMaxPiece / kWave; i++) {
-        const int d = lane + i * kWave;
-        if (d < c.npiece) a.y[row * c.npiece + d] = sum == 0.0f ? 0.0f : acc[i] / sum;
-    }
+    for (int i = 0; i < kMaxPiece / kWave; i++) sums[wave][lane + i * kWave] = acc[i];
+    __syncthreads();
+    for (int d = threadIdx.x; d < c.npiece; d += 256)
+        a.y[row * c.npiece + d] = sum == 0.0f ? 0.0f : (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) / sum;
 }
 
 int parts_buffer(Parts* parts, int64_t rows, int npiece) {
@@ -489,14 +580,14 @@ int parts_buffer(Parts* parts, int64_t rows, int npiece) {
 template <int VW, int NR>
 int launch_tiled(const CacheAttentionArgs& a, const Parts& parts, int64_t row_tiles, hipStream_t stream) {
     const CachePages& c = a.pages;
-    constexpr int lds = Tiled<VW, NR>::kLds;
-    static_assert(lds <= 160 * 1024, "LDS of a compute unit");
-    if (lds > 64 * 1024)
+    using T = Tiled<VW, NR>;
+    static_assert(T::kLds + 4 * T::kRows * 8 <= 160 * 1024, "LDS of a compute unit");
+    if (T::kLds + 4 * T::kRows * 8 > 64 * 1024)
         KAI_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_tiled_kernel<VW, NR>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds),
                           "hipFuncSetAttribute(cache_attention_tiled_kernel)"));
     const dim3 grid((unsigned)(c.nbat * c.nkvhead * row_tiles), (unsigned)parts.nsplit);
-    cache_attention_tiled_kernel<VW, NR><<<grid, 256, lds, stream>>>(a, parts, (int)row_tiles);
+    cache_attention_tiled_kernel<VW, NR><<<grid, 256, T::kLds, stream>>>(a, parts, (int)row_tiles);
     return check_launch("cache_attention_tiled_kernel");
 }
 
@@ -530,14 +621,22 @@ int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
     const int64_t reach = c.page * c.nmaxpage;
     const bool tiled = tiled_applies(a);
     const int64_t shared_rows = c.ntimes * (a.nhead / c.nkvhead);      // of a key head
-    const int nr = shared_rows <= 16 ? 1 : shared_rows <= 32 ? 2 : 4;
-    const int64_t row_tiles = (shared_rows + 16 * nr - 1) / (16 * nr);
+    const int64_t cu = compute_units();
+    const int64_t most = reach / 128 < 1 ? 1 : reach / 128 > kMaxParts ? kMaxParts : reach / 128;   // a tile for each wave
+    // The largest tile of rows that the rows fill and that leaves two workgroups for a compute unit
+    int nr = shared_rows <= 16 ? 1 : shared_rows <= 32 ? 2 : 4;
+    const auto tiles_of_rows = [&](int n) { return (shared_rows + 16 * n - 1) / (16 * n); };
+    while (nr > 1 && c.nbat * c.nkvhead * tiles_of_rows(nr) * most < 2 * cu) nr /= 2;
+    const int64_t row_tiles = tiles_of_rows(nr);
     const int64_t groups = tiled ? c.nbat * c.nkvhead * row_tiles : (rows + 3) / 4;
-    // four workgroups for a compute unit, a part of at least 256 keys
-    int64_t nsplit = (4 * (int64_t)compute_units() + groups - 1) / groups;
-    if (nsplit > reach / 256) nsplit = reach / 256;
+    const int64_t resident = nr == 4 ? 1 : 2;      // workgroups of a compute unit
+    // One round of workgroups over the chip; two where sequences of different lengths may stand side by side and the parts
+    // stay long (their workgroups then even out).  32 x 1 over 4096 to 1366 keys: one round 155 us, two 138; 1 x 16 over
+    // 131072: 294 and 314; 3 x 61 over 1500 to 834, where two rounds' parts are of 195 keys: 22.7 and 26.6.
+    int64_t nsplit = resident * cu / groups;
+    if (c.nbat > 1 && reach >= 2 * nsplit * 512) nsplit *= 2;
+    if (nsplit > most) nsplit = most;
     if (nsplit < 1) nsplit = 1;
-    if (nsplit > 256) nsplit = 256;
     Parts parts{nullptr, nullptr, (int)nsplit};
     if (nsplit > 1) KAI_TRY(parts_buffer(&parts, rows, c.npiece));
     if (tiled) {
@@ -547,7 +646,7 @@ int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
         KAI_TRY(check_launch("cache_attention_rows_kernel"));
     }
     if (nsplit == 1) return KAI_OK;
-    cache_attention_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a, parts);
+    cache_attention_join_kernel<<<(unsigned)rows, 256, 0, stream>>>(a, parts);
     return check_launch("cache_attention_join_kernel");
 }
 

@@ -17,6 +17,7 @@ namespace {
 constexpr int64_t kMaxWidth = 1ll << 24;     // floats of a token's heads
 constexpr int64_t kMaxRotary = 512;          // rotated elements of a head
 constexpr int64_t kMaxAttentionPiece = 256;
+constexpr int64_t kMaxReach = 1ll << 30;           // keys of a sequence: indices a few tiles further on still fit 32 bits
 constexpr int64_t kMaxAttentionRows = 1ll << 26;   // a wave each: the threads of a launch stay below 2^32
 
 int rotary_params(const char* who, const kai_rotary_desc* desc, int64_t npiece, RotaryParams* out) {
@@ -102,7 +103,7 @@ int cache_pages(const char* who, CachePages* c, const int* ppage, const int* ple
     if (nkvhead < 0 || npage < 0 || npagelen < 0 || nmaxpage < 0)
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": negative dimension");
     if (nkvhead > kMaxWidth || nkvhead * npiece > kMaxWidth || npage > kMaxDim || npagelen > kMaxDim || nmaxpage > kMaxDim ||
-        npagelen * nmaxpage > kMaxDim || npage * npagelen > kMaxDim)
+        npagelen * nmaxpage > kMaxReach || npage * npagelen > kMaxDim)
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": dimension out of range");
     if (ppage == nullptr && (nmaxpage > 1 || npage < nbat))
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": without a page table each sequence has one page, its own");

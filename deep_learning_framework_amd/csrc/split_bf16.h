@@ -1,41 +1,44 @@
 // fp32 products on the bf16 matrix cores without losing fp32's accuracy.
 //
-// A float is the exact sum of three bf16: x = h + m + l with h = bf16(x), m = bf16(x - h), l = x - h - m, rounded to
-// nearest, so that |m| <= 2^-8 |x|, |l| <= 2^-16 |x| and 8 + 8 + 8 bits hold all 24.  Of the nine products of two such
-// sums six are formed: hh, hm, mh, mm, hl, lh.  The three left out are below 3 * 2^-24 |x y| at most and 2^-26 |x y| in
-// the mean, what one rounding of the product costs; the products themselves are exact in the 32-bit accumulators.
+// A float is the exact sum of three bf16: h = its upper 16 bits, m = the upper 16 bits of x - h, l = x - h - m: 8 + 8 + 8
+// bits of the 24, |m| < 2^-7 |x|, |l| < 2^-15 |x|.  Of the nine products of two such sums six are formed: hh, hm, mh, mm,
+// hl, lh.  The three left out are below 2^-21 |x y| together, and in the mean 2^-24 |x y| (towards zero): half a step of
+// fp32, what rounding a product once may cost.  The products themselves are exact in the 32-bit accumulators.
+// (Pieces rounded to nearest instead would leave out 2^-26, but v_cvt_pk_bf16_f32 issues in 8 cycles where the 32-bit
+// operations here take 4 to 5: 4096 x 4096 -> 11008 3.81 ms with them, 3.67 without.)
 // v_mfma_f32_32x32x16_bf16 does 16 times the work of v_mfma_f32_32x32x2_f32 in a cycle, so six of them are 2.67 times
-// as fast as fp32 matrix instructions, for about 5.5 vector instructions per loaded float (3 conversions, 4 widenings,
-// 4 subtractions for two).  An infinity (or a value that rounds to one in bf16, above 3.39e38) becomes a NaN: callers
-// look for those.  Pieces below 2^-133 vanish, so values below 2^-109 keep fewer than 24 bits.
+// as fast as fp32 matrix instructions, for 5.5 vector instructions per loaded float (4 masks, 4 subtractions, 3 packings
+// for two).  An infinity becomes a NaN (inf - inf): callers look for those.  Pieces below 2^-133 vanish, so values below
+// 2^-109 keep fewer than 24 bits.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
 namespace kai {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 
 struct Split8 {
     bf16x8 h, m, l;
 };
 
-__device__ __forceinline__ unsigned to_bf16_pair(float a, float b) {
-    const f32x2 v = {a, b};
-    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+__device__ __forceinline__ float upper_half(float x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xFFFF0000u);
+}
+// upper halves of a (low half of the result) and b
+__device__ __forceinline__ unsigned upper_halves(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
 }
 
 __device__ __forceinline__ void split_pair(float a, float b, unsigned& h, unsigned& m, unsigned& l) {
-    h = to_bf16_pair(a, b);
-    a -= __builtin_bit_cast(float, h << 16);
-    b -= __builtin_bit_cast(float, h & 0xFFFF0000u);
-    m = to_bf16_pair(a, b);
-    a -= __builtin_bit_cast(float, m << 16);
-    b -= __builtin_bit_cast(float, m & 0xFFFF0000u);
-    l = to_bf16_pair(a, b);
+    h = upper_halves(a, b);
+    a -= upper_half(a);
+    b -= upper_half(b);
+    m = upper_halves(a, b);
+    a -= upper_half(a);
+    b -= upper_half(b);
+    l = upper_halves(a, b);
 }
 
 // eight floats x[0], x[stride], ...

@@ -433,7 +433,7 @@ int kai_rotary_backward(int device, float* pgx, const float* pgy, const int* ppo
 /* The cache.  pcK and pcV are [npage, npagelen, nkvhead * npiece] each.  Key j of sequence b is row j % npagelen of
  * page ppage[b, j / npagelen] (ppage[nbat, nmaxpage]; null: page b, nmaxpage <= 1, npage >= nbat).  A page number
  * outside [0, npage) names no page: writes to it are dropped, its keys are not seen; nor are keys at nmaxpage *
- * npagelen and behind (that product and npage * npagelen are below 2^31).  plen[nbat] is the number of keys a sequence holds already (negative: 0); the new
+ * npagelen and behind (at most 2^30; npage * npagelen is below 2^31).  plen[nbat] is the number of keys a sequence holds already (negative: 0); the new
  * ones stand behind it.  pcount[nbat], or null for ntimes, is how many of the ntimes rows of a sequence are new tokens
  * (clipped to 0 .. ntimes): the rows behind it are not read, and their results are left as they were. */
 
