@@ -56,7 +56,7 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
     p.M = a.ndat; p.N = a.yvec; p.K = (int)a.xvec;
     p.lda = p.ldb = a.xvec; p.ldc = a.yvec;
     p.nwhich = 1;
-    if (a.ndat > 32 && gated_gemm_applies(p)) return launch_gated_gemm(kGatedForward, p, stream);
+    if (a.ndat > 32 && gated_gemm_applies(kGatedForward, p)) return launch_gated_gemm(kGatedForward, p, stream);
     // both products, then the activation and the product; the pre-activations in the caller's buffers or in scratch
     const int64_t n = a.ndat * a.yvec;
     float* gate = a.gate;
@@ -78,6 +78,16 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
     return launch_gated_activation(a.y, gate, up, n, a.act, a.hleaky, stream);
 }
 
+// Gradients of up to 32 rows, and small ones, take two products of the dense layer's dispatcher each, about 7 us and
+// 65 flop a ns: their latency is lower (us with the element-wise kernel in front, two products | this file's: gx of
+// 256 x 64 -> 512 10.9 | 13.8, of 1000 x 256 -> 512 17.5 | 20.5, of 128 x 1024 -> 1024 23.3 | 19.0, of 512 x 1024 -> 1024 40.5 | 30.0; gw of
+// 512 x 64 -> 512 11.1 | 14.1, of 33 x 1024 -> 1024 14.2 | 9.9).
+static bool split_pays(int mode, const GatedGemm& p, int64_t ndat) {
+    if (ndat <= 32 || !gated_gemm_applies(mode, p)) return false;
+    const double flops = 4.0 * p.M * p.N * p.K * (mode == kGatedGw && p.nwhich == 1 ? 0.5 : 1.0);
+    return gated_gemm_us(mode, p) < 7.0 + flops / 65e6;
+}
+
 int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
     GatedGemm p{};
     p.A[0] = a.ggate; p.A[1] = a.gup;
@@ -88,7 +98,7 @@ int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
         p.C[0] = a.gx;
         p.M = a.ndat; p.N = a.xvec; p.K = (int)a.yvec;
         p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
-        if (a.ndat > 32 && gated_gemm_applies(p)) {
+        if (split_pays(kGatedGx, p, a.ndat)) {
             KAI_TRY(launch_gated_gemm(kGatedGx, p, stream));
         } else {
             KAI_TRY(kai_matmul_backward_x(0, a.gx, a.ggate, a.wg, a.yvec, a.ndat, a.xvec, a.acc));
@@ -99,17 +109,15 @@ int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
     p.B[0] = a.x; p.B[1] = nullptr;
     p.M = a.yvec; p.N = a.xvec; p.K = (int)a.ndat;
     p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
-    if (a.ndat > 32 && gated_gemm_applies(p)) {
-        p.C[0] = a.gwg; p.C[1] = a.gwu;
-        p.nwhich = 2;
-        if (a.gwg == nullptr || a.gwu == nullptr) {
-            p.nwhich = 1;
-            p.C[0] = a.gwg ? a.gwg : a.gwu;
-            p.C[1] = nullptr;
-            p.A[0] = a.gwg ? a.ggate : a.gup;
-        }
-        return launch_gated_gemm(kGatedGw, p, stream);
+    p.C[0] = a.gwg; p.C[1] = a.gwu;
+    p.nwhich = 2;
+    if (a.gwg == nullptr || a.gwu == nullptr) {
+        p.nwhich = 1;
+        p.C[0] = a.gwg ? a.gwg : a.gwu;
+        p.C[1] = nullptr;
+        p.A[0] = a.gwg ? a.ggate : a.gup;
     }
+    if (split_pays(kGatedGw, p, a.ndat)) return launch_gated_gemm(kGatedGw, p, stream);
     if (a.gwg) KAI_TRY(kai_matmul_backward_w(0, a.gwg, a.ggate, a.x, a.yvec, a.ndat, a.xvec, a.acc));
     if (a.gwu) KAI_TRY(kai_matmul_backward_w(0, a.gwu, a.gup, a.x, a.yvec, a.ndat, a.xvec, a.acc));
     return KAI_OK;

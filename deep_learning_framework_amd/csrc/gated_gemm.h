@@ -20,11 +20,14 @@ struct GatedGemm {
     int nwhich;             // gw: 2 products, or 1; otherwise 1
     // filled by the launcher
     int tiles_m, tiles_n, run, part_steps;
+    int64_t ldp;            // row length of a part's sums
     int wide;               // outputs in rows of whole 16-byte lines
     float* parts;           // partial sums of a reduction cut into parts; null: whole
 };
 
-bool gated_gemm_applies(const GatedGemm& p);
+bool gated_gemm_applies(int mode, const GatedGemm& p);
+// what the products would take, as the choice of their tiles estimates it
+double gated_gemm_us(int mode, const GatedGemm& p);
 int launch_gated_gemm(int mode, const GatedGemm& p, hipStream_t stream);
 
 }  // namespace kai

@@ -14,6 +14,8 @@
 // What lies outside an operand reads as 0 (buffer loads end with it); the last, partial step of a K-contiguous operand is
 // masked.  Where an operand held an infinity, or a value that rounds to one in bf16, sums that came out as NaN are formed
 // again in plain fp32, so that an infinity has the effect it has there.
+#include <type_traits>
+
 #include "act_funcs.h"
 #include "gated_gemm.h"
 #include "split_bf16.h"
@@ -24,6 +26,15 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// f(B), ..., f(E - 1) with compile-time indices
+template <int B, int E, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (B < E) {
+        f(std::integral_constant<int, B>{});
+        static_for<B + 1, E>(f);
+    }
+}
 
 constexpr int kStep = 16;
 constexpr int kPadRows = 8;            // between the halves of a plane: the two halves' writes meet different banks
@@ -42,52 +53,60 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_from(const float* from, c
     return __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(from), 0, (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
-// One operand's tile of ROWS rows x 16 steps.  Eight floats a thread: KC (steps contiguous): two chunks of four steps,
-// otherwise eight steps of one row.
+// One operand's tile of ROWS rows x 16 steps, F = 4 or 8 floats a thread: KC (steps contiguous): chunks of four steps,
+// otherwise F steps of one row.
 template <bool KC, int ROWS, int NT>
 struct Tile {
-    static_assert(ROWS * kStep == 8 * NT, "eight floats a thread");
+    static constexpr int F = ROWS * kStep / NT, kPieces = F / 4;
+    static_assert(F * NT == ROWS * kStep && (F == 4 || F == 8), "four or eight floats a thread");
     static constexpr int kHalf = (ROWS + kPadRows) * 16;      // bytes
     static constexpr int kPlane = 2 * kHalf;
     static constexpr int kBytes = 3 * kPlane;
 
-    // row of the tile that chunk i of this thread loads
+    // row of the tile that chunk i of this thread loads, and the first step of it
     static __device__ __forceinline__ int row_of(int i) { return KC ? ((int)threadIdx.x + i * NT) / 4 : (int)threadIdx.x % ROWS; }
+    static __device__ __forceinline__ int step_of() { return KC ? (int)threadIdx.x % 4 * 4 : (int)threadIdx.x / ROWS * F; }
 
-    static __device__ __forceinline__ void load_kc(float (&x)[8], int i, __amdgpu_buffer_rsrc_t rsrc, uint32_t off) {
+    static __device__ __forceinline__ void load_kc(float (&x)[F], int i, __amdgpu_buffer_rsrc_t rsrc, uint32_t off) {
         const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
 #pragma unroll
         for (int e = 0; e < 4; e++) x[4 * i + e] = v[e];
     }
 
     // steps from `left` on do not exist
-    static __device__ __forceinline__ void mask_kc(float (&x)[8], int left) {
-        const int q = (int)threadIdx.x % 4 * 4;
+    static __device__ __forceinline__ void mask_kc(float (&x)[F], int left) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (q + i % 4 >= left) x[i] = 0.0f;
+        for (int i = 0; i < F; i++)
+            if (step_of() + i % 4 >= left) x[i] = 0.0f;
     }
 
-    static __device__ __forceinline__ void store(char* lds, const float (&x)[8], float& largest) {
+    // Cuts and stores four of the thread's floats.  `cut` keeps what piece 0 leaves for piece 1.
+    template <int PIECE>
+    static __device__ __forceinline__ void store(char* lds, const float (&x)[F], unsigned (&cut)[6], float& largest) {
+        unsigned h[2], m[2], l[2];
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) largest = fmaxf(fmaxf(fabsf(x[i]), fabsf(x[i + 1])), largest);
-        unsigned h[4], m[4], l[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) split_pair(x[2 * i], x[2 * i + 1], h[i], m[i], l[i]);
-        if constexpr (KC) {
+        for (int i = 0; i < 2; i++) {
+            const float a = x[4 * PIECE + 2 * i], b = x[4 * PIECE + 2 * i + 1];
+            largest = fmaxf(fmaxf(fabsf(a), fabsf(b)), largest);
+            split_pair(a, b, h[i], m[i], l[i]);
+        }
+        char* to = lds + (step_of() / 8) * kHalf + row_of(PIECE) * 16;
+        if constexpr (KC || F == 4) {
+            to += step_of() % 8 * 2;
+            *reinterpret_cast<u32x2*>(to) = u32x2{h[0], h[1]};
+            *reinterpret_cast<u32x2*>(to + kPlane) = u32x2{m[0], m[1]};
+            *reinterpret_cast<u32x2*>(to + 2 * kPlane) = u32x2{l[0], l[1]};
+        } else if constexpr (PIECE == 0) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int q = (int)threadIdx.x % 4;
-                char* to = lds + (q / 2) * kHalf + row_of(i) * 16 + (q % 2) * 8;
-                *reinterpret_cast<u32x2*>(to) = u32x2{h[2 * i], h[2 * i + 1]};
-                *reinterpret_cast<u32x2*>(to + kPlane) = u32x2{m[2 * i], m[2 * i + 1]};
-                *reinterpret_cast<u32x2*>(to + 2 * kPlane) = u32x2{l[2 * i], l[2 * i + 1]};
+                cut[i] = h[i];
+                cut[2 + i] = m[i];
+                cut[4 + i] = l[i];
             }
         } else {
-            char* to = lds + ((int)threadIdx.x / ROWS) * kHalf + row_of(0) * 16;
-            *reinterpret_cast<u32x4v*>(to) = u32x4v{h[0], h[1], h[2], h[3]};
-            *reinterpret_cast<u32x4v*>(to + kPlane) = u32x4v{m[0], m[1], m[2], m[3]};
-            *reinterpret_cast<u32x4v*>(to + 2 * kPlane) = u32x4v{l[0], l[1], l[2], l[3]};
+            *reinterpret_cast<u32x4v*>(to) = u32x4v{cut[0], cut[1], h[0], h[1]};
+            *reinterpret_cast<u32x4v*>(to + kPlane) = u32x4v{cut[2], cut[3], m[0], m[1]};
+            *reinterpret_cast<u32x4v*>(to + 2 * kPlane) = u32x4v{cut[4], cut[5], l[0], l[1]};
         }
     }
 
@@ -100,15 +119,18 @@ struct Tile {
     }
 };
 
-// The plain sum of one output, for sums that an infinity entered: the reduction steps [s0, s1) of the launch
+// The plain sum of one output over what this workgroup reduces (whole steps [s0, s1), and the rests behind the whole steps
+// where it has them), for sums that an infinity entered.
 template <int MODE>
-__device__ float plain_sum(const GatedGemm& p, int which, int64_t m, int64_t n, int s0, int s1) {
+__device__ float plain_sum(const GatedGemm& p, int which, int64_t m, int64_t n, int s0, int s1, bool rests) {
     float sum = 0.0f;
-    const int steps = (p.K + kStep - 1) / kStep;
-    for (int s = s0; s < s1; s++) {
-        const int seg = MODE == kGatedGx && s >= steps ? 1 : 0;
-        const int k0 = (s - seg * steps) * kStep;
-        for (int k = k0; k < k0 + kStep && k < p.K; k++) {
+    const int full = p.K / kStep;
+    for (int seg = 0; seg < (MODE == kGatedGx ? 2 : 1); seg++) {
+        const int from = s0 - seg * full, to = s1 - seg * full;
+        const int k0 = (from < 0 ? 0 : from > full ? full : from) * kStep;
+        const int k1 = (to < 0 ? 0 : to > full ? full : to) * kStep;
+        for (int k = k0; k < p.K; k++) {
+            if (k >= k1 && (!rests || k < full * kStep)) continue;
             if (MODE == kGatedForward) sum = fmaf(p.A[0][m * p.lda + k], p.B[which][n * p.ldb + k], sum);
             if (MODE == kGatedGx) sum = fmaf(p.A[seg][m * p.lda + k], p.B[seg][k * p.ldb + n], sum);
             if (MODE == kGatedGw) sum = fmaf(p.A[which][k * p.lda + m], p.B[0][k * p.ldb + n], sum);
@@ -130,6 +152,40 @@ __device__ __forceinline__ void put(float* row, int64_t n, int64_t N, const f32x
     }
 }
 
+template <int ACT>
+__device__ __forceinline__ f32x4 activate_as(const f32x4& x, float leaky) {
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = apply_act(x[e], ACT, leaky);
+    return y;
+}
+
+// one jump for four values
+__device__ __forceinline__ f32x4 activate4(const f32x4& x, int act, float leaky) {
+    switch (act) {
+    case kActRelu: return activate_as<kActRelu>(x, leaky);
+    case kActLeaky: return activate_as<kActLeaky>(x, leaky);
+    case kActSigmoid: return activate_as<kActSigmoid>(x, leaky);
+    case kActTanh: return activate_as<kActTanh>(x, leaky);
+    case kActGelu: return activate_as<kActGelu>(x, leaky);
+    case kActSelu: return activate_as<kActSelu>(x, leaky);
+    case kActMish: return activate_as<kActMish>(x, leaky);
+    case kActSwish: return activate_as<kActSwish>(x, leaky);
+    default: return x;
+    }
+}
+
+// bias[n .. n + 3], 0 where there is none
+__device__ __forceinline__ f32x4 bias4(const float* bias, int64_t n, int64_t N) {
+    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (bias) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < N) b[e] = bias[n + e];
+    }
+    return b;
+}
+
 template <int MODE, int WM, int WN, int NBM>
 struct Shape {
     static constexpr int NBN = 2;
@@ -144,7 +200,7 @@ struct Shape {
 };
 
 template <int MODE, int WM, int WN, int NBM>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p) {
+__global__ __launch_bounds__(64 * WM * WN, NBM == 4 ? 2 : NBM == 2 ? 3 : 4) void gated_gemm_kernel(GatedGemm p) {
     using S = Shape<MODE, WM, WN, NBM>;
     using TA = typename S::TA;
     using TB = typename S::TB;
@@ -170,61 +226,86 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
         tn = in / rows;
     }
     const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * S::kColumns;
-    const int steps = (p.K + kStep - 1) / kStep, all_steps = MODE == kGatedGx ? 2 * steps : steps;
+    // Whole steps [s0, s1) of this part of the reduction; the last part takes the rests (K % 16 steps a segment) as well.
+    constexpr int kSegments = MODE == kGatedGx ? 2 : 1;
+    const int full = p.K / kStep;
     const int s0 = (int)blockIdx.y * p.part_steps;
-    const int s1 = s0 + p.part_steps < all_steps ? s0 + p.part_steps : all_steps;
+    const int s1 = s0 + p.part_steps < kSegments * full ? s0 + p.part_steps : kSegments * full;
+    const bool rests = blockIdx.y + 1 == gridDim.y && p.K % kStep != 0;
 
-    // byte offsets of this thread's rows from the tile's first row
-    uint32_t aoff[2], boff[2];
+    // Buffers that end with the operands.  K-contiguous operands start at the tile's first row, the others at its first
+    // column and, with one segment, at the part's first step: offsets inside stay below 4 GiB.
+    const int64_t astart = S::AKC ? m0 * p.lda : m0 + (kSegments == 1 ? (int64_t)s0 * kStep * p.lda : 0);
+    const int64_t bstart = S::BKC ? n0 * p.ldb : n0 + (kSegments == 1 ? (int64_t)s0 * kStep * p.ldb : 0);
+    const int64_t aend = S::AKC ? (p.M - 1) * p.lda + p.K : (p.K - 1) * p.lda + p.M;
+    const int64_t bend = S::BKC ? (p.N - 1) * p.ldb + p.K : (p.K - 1) * p.ldb + p.N;
+    __amdgpu_buffer_rsrc_t arsrc[kSegments], brsrc[2];
+    // byte offsets of this thread's loads of step 0 from there
+    uint32_t aoff[2], boff[2];       // (a transposing thread's other loads are rows further on)
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        aoff[i] = S::AKC ? (uint32_t)((TA::row_of(i) * p.lda + (int)threadIdx.x % 4 * 4) * 4) : (uint32_t)TA::row_of(0) * 4;
-        boff[i] = S::BKC ? (uint32_t)((TB::row_of(i) % 32 + TB::row_of(i) / 64 * 32) * p.ldb + (int)threadIdx.x % 4 * 4) * 4
-                         : (uint32_t)TB::row_of(0) * 4;
+    for (int g = 0; g < kSegments; g++) {
+        const float* A = MODE == kGatedGw ? p.A[which] : p.A[g];
+        arsrc[g] = rsrc_from(A + astart, A + aend);
     }
-    float xa[8], xb[8];
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        // forward: rows of the tile alternate between the weights, 32 at a time, so a load's rows are of one of them
+        const float* B = MODE == kGatedForward ? p.B[__builtin_amdgcn_readfirstlane(TB::row_of(g) / 32 % 2)] : p.B[g < kSegments ? g : 0];
+        brsrc[g] = rsrc_from(B + bstart, B + bend);
+    }
+    if constexpr (S::AKC) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) aoff[i] = (uint32_t)(TA::row_of(i) * p.lda + TA::step_of()) * 4;
+    } else {
+        aoff[0] = (uint32_t)(TA::step_of() * p.lda + TA::row_of(0)) * 4;
+    }
+    if constexpr (S::BKC) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            boff[i] = (uint32_t)((TB::row_of(i) % 32 + TB::row_of(i) / 64 * 32) * p.ldb + TB::step_of()) * 4;
+    } else {
+        boff[0] = (uint32_t)(TB::step_of() * p.ldb + TB::row_of(0)) * 4;
+    }
+    float xa[2][TA::F], xb[2][TB::F];     // of the next step and of the one after it
     float largest = 0.0f;
-    const auto load = [&](int s) {
-        const int seg = MODE == kGatedGx && s >= steps ? 1 : 0;
-        const int64_t k0 = (int64_t)(s - seg * steps) * kStep;
-        const float* A = MODE == kGatedGx ? p.A[seg] : MODE == kGatedGw ? p.A[which] : p.A[0];
+    // 16 steps of a segment from step s on
+    const auto load_steps = [&](int segment, int s, auto set) {
+        constexpr int q = decltype(set)::value;
+        const auto ar = segment == 0 ? arsrc[0] : arsrc[kSegments - 1];
+        const uint32_t from = (uint32_t)(kSegments == 1 ? s - s0 : s) * kStep * 4;      // of an operand that starts there
+        const uint32_t ka = S::AKC ? (uint32_t)s * kStep * 4 : from * (uint32_t)p.lda;
+        const uint32_t kb = S::BKC ? (uint32_t)s * kStep * 4 : from * (uint32_t)p.ldb;
         if constexpr (S::AKC) {
-            const auto rsrc = rsrc_from(A + m0 * p.lda + k0, A + (p.M - 1) * p.lda + p.K);
 #pragma unroll
-            for (int i = 0; i < 2; i++) TA::load_kc(xa, i, rsrc, aoff[i]);
+            for (int i = 0; i < TA::kPieces; i++) TA::load_kc(xa[q], i, ar, aoff[i] + ka);
         } else {
-            const auto rsrc = rsrc_from(A + k0 * p.lda + m0, A + (p.K - 1) * p.lda + p.M);
-            const uint32_t oct = (uint32_t)threadIdx.x / S::BM * 8;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                xa[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, aoff[0] + (oct + i) * (uint32_t)(p.lda * 4), 0, 0));
+            for (int i = 0; i < TA::F; i++)
+                xa[q][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(ar, aoff[0] + (ka + (uint32_t)i * (uint32_t)p.lda * 4), 0, 0));
         }
         if constexpr (S::BKC) {
-            // rows of the tile alternate between the weights, 32 at a time
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int w = __builtin_amdgcn_readfirstlane(TB::row_of(i) / 32 % 2);
-                const float* B = p.B[w];
-                TB::load_kc(xb, i, rsrc_from(B + n0 * p.ldb + k0, B + (p.N - 1) * p.ldb + p.K), boff[i]);
-            }
+            for (int i = 0; i < TB::kPieces; i++) TB::load_kc(xb[q], i, brsrc[i], boff[i] + kb);
         } else {
-            const float* B = p.B[seg];
-            const auto rsrc = rsrc_from(B + k0 * p.ldb + n0, B + (p.K - 1) * p.ldb + p.N);
-            const uint32_t oct = (uint32_t)threadIdx.x / S::BN * 8;
+            const auto br = segment == 0 ? brsrc[0] : brsrc[kSegments - 1];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                xb[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, boff[0] + (oct + i) * (uint32_t)(p.ldb * 4), 0, 0));
-        }
-        const int left = p.K - (int)k0;
-        if (left < kStep) {
-            if constexpr (S::AKC) TA::mask_kc(xa, left);
-            if constexpr (S::BKC) TB::mask_kc(xb, left);
+            for (int i = 0; i < TB::F; i++)
+                xb[q][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(br, boff[0] + (kb + (uint32_t)i * (uint32_t)p.ldb * 4), 0, 0));
         }
     };
-    const auto store = [&](int buffer) {
-        char* to = lds + buffer * (TA::kBytes + TB::kBytes);
-        TA::store(to, xa, largest);
-        TB::store(to + TA::kBytes, xb, largest);
+    // whole step s of the reduction
+    const auto load = [&](int s, auto set) {
+        const int segment = kSegments == 2 && s >= full ? 1 : 0;
+        load_steps(segment, s - segment * full, set);
+    };
+    unsigned cut_a[6], cut_b[6];
+    // part PIECE of the step's cutting and storing
+    constexpr int kPieces = TA::kPieces + TB::kPieces;
+    const auto store = [&](auto set, auto piece) {
+        constexpr int q = decltype(set)::value, PIECE = decltype(piece)::value;
+        char* to = lds + q * (TA::kBytes + TB::kBytes);
+        if constexpr (PIECE < TA::kPieces) TA::template store<PIECE>(to, xa[q], cut_a, largest);
+        else TB::template store<PIECE - TA::kPieces>(to + TA::kBytes, xb[q], cut_b, largest);
     };
 
     f32x16 acc[NBM][NBN];
@@ -235,21 +316,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
 
-    if (s0 < s1) {
-        load(s0);
-        store(0);
-    }
-    __syncthreads();
-    for (int s = s0; s < s1; s++) {
-        const bool more = s + 1 < s1;
-        if (more) load(s + 1);
-        const char* from = lds + (s - s0) % 2 * (TA::kBytes + TB::kBytes);
+    const int pairs_end = s1 > s0 ? s0 + (s1 - s0) / 2 * 2 : s0;     // steps go in pairs, the last odd one by itself
+    // the products of a buffer's step; between(i) runs behind those of the wave's i-th 32 rows
+    const auto products = [&](const char* from, auto between) {
         Split8 b[NBN];
 #pragma unroll
         for (int j = 0; j < NBN; j++) b[j] = TB::fragment(from + TA::kBytes, wn * 32 * NBN + 32 * j);
-#pragma unroll
-        for (int i = 0; i < NBM; i++) {
-            const Split8 a = TA::fragment(from, wm * 32 * NBM + 32 * i);
+        Split8 next = TA::fragment(from, wm * 32 * NBM);
+        static_for<0, NBM>([&](auto block) {
+            constexpr int i = decltype(block)::value;
+            const Split8 a = next;
+            if constexpr (i + 1 < NBM) next = TA::fragment(from, wm * 32 * NBM + 32 * (i + 1));
             // the small products first
 #pragma unroll
             for (int j = 0; j < NBN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b[j].l, acc[i][j], 0, 0, 0);
@@ -263,8 +340,47 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
             for (int j = 0; j < NBN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b[j].h, acc[i][j], 0, 0, 0);
 #pragma unroll
             for (int j = 0; j < NBN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b[j].h, acc[i][j], 0, 0, 0);
+            between(block);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // A step: the loads of two steps further on (in front, or the scheduler sinks them to their use), the products of this
+    // one, and between them the cutting of the next.  What is loaded and cut behind the last step is its data once more, and
+    // not used.
+    const auto step = [&](int s, auto set) {
+        constexpr int q = decltype(set)::value;
+        load(s + 2 < pairs_end ? s + 2 : pairs_end - 1, set);
+        __builtin_amdgcn_sched_barrier(0);
+        products(lds + q * (TA::kBytes + TB::kBytes), [&](auto block) {
+            constexpr int i = decltype(block)::value;
+            static_for<kPieces * i / NBM, kPieces * (i + 1) / NBM>([&](auto piece) { store(std::integral_constant<int, 1 - q>{}, piece); });
+        });
+        __syncthreads();
+    };
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    if (s0 < pairs_end) {
+        load(s0, Zero{});
+        load(s0 + 1, One{});
+        static_for<0, kPieces>([&](auto piece) { store(Zero{}, piece); });
+        __syncthreads();
+        for (int s = s0; s < pairs_end; s += 2) {
+            step(s, Zero{});
+            step(s + 1, One{});
         }
-        if (more) store((s + 1 - s0) % 2);
+    }
+    // the odd step, and the rests of the segments
+    const int odd = s1 > pairs_end ? 1 : 0, tail = odd + (rests ? kSegments : 0);
+#pragma unroll 1
+    for (int i = 0; i < tail; i++) {
+        const int segment = i < odd ? (kSegments == 2 && pairs_end >= full ? 1 : 0) : i - odd;
+        load_steps(segment, i < odd ? pairs_end - segment * full : full, Zero{});
+        const int left = i < odd ? kStep : p.K % kStep;
+        if constexpr (S::AKC) TA::mask_kc(xa[0], left);
+        if constexpr (S::BKC) TB::mask_kc(xb[0], left);
+        static_for<0, kPieces>([&](auto piece) { store(Zero{}, piece); });
+        __syncthreads();
+        products(lds, [](auto) {});
         __syncthreads();
     }
 
@@ -273,6 +389,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
     const bool again = __syncthreads_or(!(largest < kBf16Limit));
     const float leaky = MODE == kGatedForward && p.hleaky ? *p.hleaky : 0.0f;
     float* stage = reinterpret_cast<float*>(lds) + wave * S::kStageFloats;
+    const int64_t n = n0 + wn * (MODE == kGatedForward ? 32 : 64) + lane % 8 * 4;      // this lane's columns,
+    const int64_t n2 = MODE == kGatedForward ? n : n + 32;                           // and the other block's
+    f32x4 bg, bu;
+    if (MODE == kGatedForward && p.parts == nullptr) {
+        bg = bias4(p.bias[0], n, p.N);
+        bu = bias4(p.bias[1], n, p.N);
+    }
 #pragma unroll
     for (int i = 0; i < NBM; i++) {
         __builtin_amdgcn_wave_barrier();
@@ -282,38 +405,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
             for (int e = 0; e < 16; e++)
                 stage[(8 * (e / 4) + 4 * (lane >> 5) + e % 4) * kStageRow + 32 * j + (lane & 31)] = acc[i][j][e];
         __builtin_amdgcn_wave_barrier();
+        if (again) {
+#pragma unroll 1
+            for (int e = lane; e < 32 * 64; e += 64) {
+                const int r = e / 64, c = e % 64;
+                float* x = stage + r * kStageRow + c;
+                const int64_t m = m0 + wm * 32 * NBM + 32 * i + r;
+                const int64_t col = MODE == kGatedForward ? n0 + wn * 32 + c % 32 : n0 + wn * 64 + c;
+                if (*x != *x && m < p.M && col < p.N) *x = plain_sum<MODE>(p, MODE == kGatedForward ? c / 32 : which, m, col, s0, s1, rests);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll 1
         for (int r = lane / 8; r < 32; r += 8) {
             const int64_t m = m0 + wm * 32 * NBM + 32 * i + r;
             if (m >= p.M) break;
             const float* row = stage + r * kStageRow + lane % 8 * 4;
             f32x4 v = *reinterpret_cast<const f32x4*>(row), u = *reinterpret_cast<const f32x4*>(row + 32);
-            const int c = lane % 8 * 4;
-            const int64_t n = n0 + wn * (MODE == kGatedForward ? 32 : 64) + c;
-            const int64_t n2 = MODE == kGatedForward ? n : n + 32;
-            if (again) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (v[e] != v[e] && n + e < p.N) v[e] = plain_sum<MODE>(p, which, m, n + e, s0, s1);
-                    if (u[e] != u[e] && n2 + e < p.N) u[e] = plain_sum<MODE>(p, MODE == kGatedForward ? 1 : which, m, n2 + e, s0, s1);
-                }
-            }
             const int64_t at = m * p.ldc;
             if constexpr (MODE == kGatedForward) {
                 if (p.parts) {
-                    float* part = p.parts + (int64_t)blockIdx.y * 2 * p.M * p.ldc + at;
-                    put(part, n, p.N, v, p.wide);
-                    put(part + p.M * p.ldc, n, p.N, u, p.wide);
+                    float* part = p.parts + ((int64_t)blockIdx.y * 2 * p.M + m) * p.ldp;
+                    put(part, n, p.ldp, v, 1);
+                    put(part + p.M * p.ldp, n, p.ldp, u, 1);
                 } else {
-                    f32x4 y;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (n + e < p.N) {
-                            v[e] += p.bias[0] ? p.bias[0][n + e] : 0.0f;
-                            u[e] += p.bias[1] ? p.bias[1][n + e] : 0.0f;
-                        }
-                        y[e] = apply_act(v[e], p.act, leaky) * u[e];
-                    }
+                    v += bg;
+                    u += bu;
+                    const f32x4 y = activate4(v, p.act, leaky) * u;
                     if (p.C[1]) {
                         put(p.C[1] + at, n, p.N, v, p.wide);
                         put(p.C[2] + at, n, p.N, u, p.wide);
@@ -321,9 +439,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
                     put(p.C[0] + at, n, p.N, y, p.wide);
                 }
             } else if (p.parts) {
-                float* part = p.parts + ((int64_t)blockIdx.y * p.nwhich + which) * p.M * p.ldc + at;
-                put(part, n, p.N, v, p.wide);
-                put(part, n2, p.N, u, p.wide);
+                float* part = p.parts + (((int64_t)blockIdx.y * p.nwhich + which) * p.M + m) * p.ldp;
+                put(part, n, p.ldp, v, 1);
+                put(part, n2, p.ldp, u, 1);
             } else {
                 float* c0 = p.C[which] + at;
                 if (p.acc) {
@@ -340,31 +458,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gated_gemm_kernel(GatedGemm p
     }
 }
 
-// sums the parts, with the forward's epilogue or onto the gradient
+// Sums the parts (rows of whole 16-byte lines, four columns a thread), with the forward's epilogue or onto the gradient.
 template <int MODE>
 __global__ __launch_bounds__(256) void gated_parts_kernel(GatedGemm p, int nparts) {
-    const int64_t one = p.M * p.ldc, total = one * (MODE == kGatedForward ? 1 : p.nwhich);
+    const int lines = (int)(p.ldp / 4);
+    const int64_t one = p.M * lines, total = one * (MODE == kGatedForward ? 1 : p.nwhich);
     const int64_t all = one * (MODE == kGatedForward ? 2 : p.nwhich);
     const float leaky = MODE == kGatedForward && p.hleaky ? *p.hleaky : 0.0f;
+    const f32x4* parts = reinterpret_cast<const f32x4*>(p.parts);
     for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        float v = 0.0f, u = 0.0f;
-        for (int s = 0; s < nparts; s++) {
-            v += p.parts[s * all + e];
-            if (MODE == kGatedForward) u += p.parts[s * all + one + e];
+        f32x4 v = parts[e], u = MODE == kGatedForward ? parts[one + e] : v;
+#pragma unroll 4
+        for (int s = 1; s < nparts; s++) {
+            v += parts[s * all + e];
+            if (MODE == kGatedForward) u += parts[s * all + one + e];
         }
+        const int which = MODE == kGatedForward ? 0 : (int)(e / one);
+        const int64_t m = (e - which * one) / lines, n = (e - which * one - m * lines) * 4;
+        const int64_t at = m * p.ldc;
         if constexpr (MODE == kGatedForward) {
-            const int64_t n = e % p.ldc;
-            v += p.bias[0] ? p.bias[0][n] : 0.0f;
-            u += p.bias[1] ? p.bias[1][n] : 0.0f;
+            v += bias4(p.bias[0], n, p.N);
+            u += bias4(p.bias[1], n, p.N);
+            const f32x4 y = activate4(v, p.act, leaky) * u;
             if (p.C[1]) {
-                p.C[1][e] = v;
-                p.C[2][e] = u;
+                put(p.C[1] + at, n, p.N, v, p.wide);
+                put(p.C[2] + at, n, p.N, u, p.wide);
             }
-            p.C[0][e] = apply_act(v, p.act, leaky) * u;
+            put(p.C[0] + at, n, p.N, y, p.wide);
         } else {
-            const int which = (int)(e / one);
-            float* c = p.C[which] + (e - which * one);
-            *c = p.acc ? *c + v : v;
+            float* c = p.C[which] + at;
+            if (p.acc) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (n + i < p.N) v[i] += c[n + i];
+            }
+            put(c, n, p.N, v, p.wide);
         }
     }
 }
@@ -379,43 +507,78 @@ int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
         KAI_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_gemm_kernel<MODE, WM, WN, NBM>),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds),
                           "hipFuncSetAttribute(gated_gemm_kernel)"));
-    const int steps = (int)((p.K + kStep - 1) / kStep) * (MODE == kGatedGx ? 2 : 1);
-    p.part_steps = (int)((steps + nparts - 1) / nparts);
+    const int steps = p.K / kStep * (MODE == kGatedGx ? 2 : 1);
+    p.part_steps = (int)((steps + nparts - 1) / nparts + 1) / 2 * 2;
     nparts = p.part_steps > 0 ? (steps + p.part_steps - 1) / p.part_steps : 1;
+    p.ldp = (p.N + 3) / 4 * 4;
     if (nparts > 1) {
-        const int64_t outputs = p.M * p.ldc * (MODE == kGatedForward ? 2 : p.nwhich);
+        const int64_t outputs = p.M * p.ldp * (MODE == kGatedForward ? 2 : p.nwhich);
         KAI_TRY(workspace(nparts * outputs * (int64_t)sizeof(float), &p.parts));
     }
     p.wide = p.ldc % 4 == 0 && aligned16(p.C[0]) && aligned16(p.C[1]) && aligned16(p.C[2]);
-    if (p.parts) p.wide = p.ldc % 4 == 0 && p.M * p.ldc % 4 == 0;
     const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.nwhich), (unsigned)nparts);
     gated_gemm_kernel<MODE, WM, WN, NBM><<<grid, S::NT, S::kLds, stream>>>(p);
     KAI_TRY(check_launch("gated_gemm_kernel"));
     if (nparts == 1) return KAI_OK;
-    const int64_t groups = (p.M * p.ldc * p.nwhich + 255) / 256, most = 16 * (int64_t)compute_units();
+    const int64_t groups = (p.M * p.ldp / 4 * p.nwhich + 255) / 256, most = 16 * (int64_t)compute_units();
     gated_parts_kernel<MODE><<<(unsigned)(groups < most ? groups : most), 256, 0, stream>>>(p, (int)nparts);
     return check_launch("gated_parts_kernel");
 }
 
+// The tile and the parts of the reduction that this estimate (us) finds cheapest.  A workgroup's step of 16 takes 0.42
+// (64 x 128 tiles), 0.70 (128 x 128) or 2.35 (256 x 256), the workgroups of a compute unit one after another (the small
+// tiles' run side by side, but share the matrix cores); its start and epilogue `fixed`; parts a launch of 4 and their sums
+// written and read at 10 bytes a ns.  Fitted to 35 shapes, 33 to 2048 rows by 64 to 4096 by 333 to 4096, against 1, 2, 3, 4, 6,
+// 8, 12 and 16 parts of each tile: within a tenth of the fastest for all but a few.  The sides, in us: 1000 x 777 -> 333 20.3 with two
+// parts of 64 x 128, 22.0 with four of 128 x 128; 512 x 1024 -> 4096 55 with 128 x 128, 58 with 64 x 128; 2048 x 1024 -> 4096 165 with
+// 256 x 256, 184 with 128 x 128; 256 x 4096 -> 4096 99 with eight parts of 256 x 256, 121 with 64 x 128 whole.
+struct Plan {
+    int tile = 0;      // 0: 64 x 128, 1: 128 x 128, 2: 256 x 256
+    int parts = 1;
+    double us = 1e30;
+};
+
+template <int MODE>
+Plan plan_of(const GatedGemm& p) {
+    constexpr int rows[3] = {64, 128, 256}, columns[3] = {128, 128, 256};
+    constexpr double step[3] = {0.42, 0.70, 2.35};
+    constexpr double fixed_forward[3] = {7.7, 12.0, 19.0}, fixed_gradient[3] = {5.2, 6.5, 14.0};
+    const int64_t all_columns = MODE == kGatedForward ? 2 * p.N : p.N, cu = compute_units();
+    const int64_t steps = (p.K + kStep - 1) / kStep * (MODE == kGatedGx ? 2 : 1);
+    Plan best;
+    for (int t = 0; t < 3; t++) {
+        const int64_t tiles = (p.M + rows[t] - 1) / rows[t] * ((all_columns + columns[t] - 1) / columns[t]) * p.nwhich;
+        for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (parts > 1 && steps < 4 * parts) break;
+            const int64_t each = ((steps + parts - 1) / parts + 1) / 2 * 2, rounds = (tiles * parts + cu - 1) / cu;
+            double us = (MODE == kGatedForward ? fixed_forward : fixed_gradient)[t] + (double)(rounds * each) * step[t];
+            if (parts > 1) us += 4.0 + parts * (double)(p.M * all_columns * p.nwhich) * 8.0 / 1e7;
+            if (us < best.us) best = Plan{t, parts, us};
+        }
+    }
+    return best;
+}
+
 template <int MODE>
 int launch_mode(const GatedGemm& p, hipStream_t stream) {
-    const int64_t columns = MODE == kGatedForward ? 2 * p.N : p.N;
-    const auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((columns + b - 1) / b) * p.nwhich; };
-    const int64_t cu = compute_units();
-    if (tiles(256) >= cu) return launch_shape<MODE, 2, 4, 4>(p, 1, stream);
-    int64_t nparts = (2 * cu) / tiles(128);
-    const int64_t steps = (p.K + kStep - 1) / kStep * (MODE == kGatedGx ? 2 : 1);
-    if (nparts > steps / 16) nparts = steps / 16;
-    if (nparts < 1) nparts = 1;
-    if (nparts > 16) nparts = 16;
-    return launch_shape<MODE, 2, 2, 2>(p, nparts, stream);
+    const Plan plan = plan_of<MODE>(p);
+    if (plan.tile == 0) return launch_shape<MODE, 2, 2, 1>(p, plan.parts, stream);
+    if (plan.tile == 1) return launch_shape<MODE, 2, 2, 2>(p, plan.parts, stream);
+    return launch_shape<MODE, 2, 4, 4>(p, plan.parts, stream);
 }
 
 }  // namespace
 
-// offsets inside a tile are 32-bit
-bool gated_gemm_applies(const GatedGemm& p) {
-    return p.M > 0 && p.N > 0 && p.K > 0 && p.lda < (1ll << 21) && p.ldb < (1ll << 21);
+// Offsets inside a workgroup's operands are 32-bit: 256 rows of a K-contiguous operand, all steps of another.
+bool gated_gemm_applies(int mode, const GatedGemm& p) {
+    if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.lda >= (1ll << 21) || p.ldb >= (1ll << 21)) return false;
+    const int64_t rows = (int64_t)p.K + kStep;
+    if (mode != kGatedForward && rows * p.ldb >= (1ll << 30)) return false;
+    return mode != kGatedGw || rows * p.lda < (1ll << 30);
+}
+
+double gated_gemm_us(int mode, const GatedGemm& p) {
+    return mode == kGatedForward ? plan_of<kGatedForward>(p).us : mode == kGatedGx ? plan_of<kGatedGx>(p).us : plan_of<kGatedGw>(p).us;
 }
 
 int launch_gated_gemm(int mode, const GatedGemm& p, hipStream_t stream) {
