@@ -81,6 +81,9 @@ struct GatedArgs {
     const float* hleaky;
 };
 int launch_gated_forward(const GatedArgs& a, hipStream_t stream);
+// up to 32 rows in one launch (gated_rows.hip), where that is the faster way
+bool gated_rows_pays(const GatedArgs& a);
+int launch_gated_rows(const GatedArgs& a, hipStream_t stream);
 
 struct GatedGradArgs {
     float* gx;              // any of the three may be null
@@ -97,9 +100,11 @@ struct GatedGradArgs {
 // gx (+)= ggate . wg + gup . wu, gwg (+)= ggate^T . x, gwu (+)= gup^T . x
 int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream);
 
-// ggate = gy * up * act'(gate), gup = gy * act(gate), n elements each
-int launch_gated_activation_backward(float* ggate, float* gup, const float* gy, const float* gate, const float* up,
-                                     int64_t n, int act, const float* hleaky, hipStream_t stream);
+// ggate = gy * up * act'(gate), gup = gy * act(gate), [nrow, ncol] each, and their column sums gbg, gbu (+= with acc; null:
+// not wanted)
+int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float* gbu, const float* gy, const float* gate,
+                                     const float* up, int64_t nrow, int64_t ncol, int act, const float* hleaky, int acc,
+                                     hipStream_t stream);
 // y = act(gate) * up
 int launch_gated_activation(float* y, const float* gate, const float* up, int64_t n, int act, const float* hleaky,
                             hipStream_t stream);

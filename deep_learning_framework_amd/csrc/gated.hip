@@ -1,6 +1,7 @@
 // The gated feed-forward projection: y = act(x . wg^T + bg) * (x . wu^T + bu), and its element-wise gradients.
 #include "act_funcs.h"
 #include "decoder_ops.h"
+#include "elementwise.h"
 #include "gated_gemm.h"
 #include "gemm_host.h"
 
@@ -16,16 +17,76 @@ __global__ __launch_bounds__(kThreads) void gated_activation_kernel(float* y, co
         y[i] = apply_act(gate[i], act, leaky) * up[i];
 }
 
-__global__ __launch_bounds__(kThreads) void gated_activation_backward_kernel(float* ggate, float* gup, const float* gy,
-                                                                             const float* gate, const float* up, int64_t n,
-                                                                             int act, const float* hleaky) {
+// ggate = gy * up * act'(gate), gup = gy * act(gate) and, on the way, their column sums: a workgroup takes 64 * VEC columns of
+// `chunk` rows, a wave every fourth of them, and leaves the sums of its rows in sums[2][chunks][ncol] (null: no sums wanted).
+// Bound: HBM, five floats an element; the sums cost nothing beside that, where sums of the stored gradients would read
+// two of the five again.
+template <int VEC>
+__global__ __launch_bounds__(kThreads) void gated_activation_backward_kernel(float* ggate, float* gup, float* sums, const float* gy,
+                                                                             const float* gate, const float* up, int64_t nrow,
+                                                                             int64_t ncol, int chunk, int act,
+                                                                             const float* hleaky) {
+    typedef float vec __attribute__((ext_vector_type(VEC)));
+    __shared__ float meet[3][2][64 * VEC];
     const float leaky = hleaky ? *hleaky : 0.0f;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-        const float g = gate[i], d = gy[i];
-        const float u = up[i];
-        ggate[i] = d * u * act_derivative(g, act, leaky);
-        gup[i] = d * apply_act(g, act, leaky);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * VEC, r0 = (int64_t)blockIdx.y * chunk;
+    const int64_t r1 = r0 + chunk < nrow ? r0 + chunk : nrow;
+    float sg[VEC] = {}, su[VEC] = {};
+    if (c < ncol) {
+        for (int64_t r = r0 + wave; r < r1; r += 4) {
+            const int64_t at = r * ncol + c;
+            const vec d = *reinterpret_cast<const vec*>(gy + at), g = *reinterpret_cast<const vec*>(gate + at);
+            const vec u = *reinterpret_cast<const vec*>(up + at);
+            vec a, b;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                a[e] = d[e] * u[e] * act_derivative(g[e], act, leaky);
+                b[e] = d[e] * apply_act(g[e], act, leaky);
+                sg[e] += a[e];
+                su[e] += b[e];
+            }
+            *reinterpret_cast<vec*>(ggate + at) = a;
+            *reinterpret_cast<vec*>(gup + at) = b;
+        }
     }
+    if (sums == nullptr) return;
+    if (wave > 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            meet[wave - 1][0][lane * VEC + e] = sg[e];
+            meet[wave - 1][1][lane * VEC + e] = su[e];
+        }
+    }
+    __syncthreads();
+    if (wave > 0 || c >= ncol) return;
+    float* to = sums + (int64_t)blockIdx.y * ncol + c;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        to[e] = sg[e] + meet[0][0][lane * VEC + e] + meet[1][0][lane * VEC + e] + meet[2][0][lane * VEC + e];
+        to[(int64_t)gridDim.y * ncol + e] = su[e] + meet[0][1][lane * VEC + e] + meet[1][1][lane * VEC + e] + meet[2][1][lane * VEC + e];
+    }
+}
+
+// gb (+)= the chunks' sums: 64 columns a workgroup, every fourth chunk a wave; blockIdx.y: gate or up
+__global__ __launch_bounds__(kThreads) void gated_bias_kernel(float* gbg, float* gbu, const float* sums, int64_t ncol, int chunks,
+                                                              int acc) {
+    __shared__ float meet[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float* gb = blockIdx.y ? gbu : gbg;
+    if (gb == nullptr) return;
+    const float* from = sums + (int64_t)blockIdx.y * chunks * ncol + c;
+    float sum = 0.0f;
+    if (c < ncol) {
+#pragma unroll 8
+        for (int i = wave; i < chunks; i += 4) sum += from[i * ncol];
+    }
+    if (wave > 0) meet[wave - 1][lane] = sum;
+    __syncthreads();
+    if (wave > 0 || c >= ncol) return;
+    sum += meet[0][lane] + meet[1][lane] + meet[2][lane];
+    gb[c] = acc ? gb[c] + sum : sum;
 }
 
 unsigned grid_of(int64_t n) {
@@ -41,10 +102,36 @@ int launch_gated_activation(float* y, const float* gate, const float* up, int64_
     return check_launch("gated_activation_kernel");
 }
 
-int launch_gated_activation_backward(float* ggate, float* gup, const float* gy, const float* gate, const float* up,
-                                     int64_t n, int act, const float* hleaky, hipStream_t stream) {
-    gated_activation_backward_kernel<<<grid_of(n), kThreads, 0, stream>>>(ggate, gup, gy, gate, up, n, act, hleaky);
-    return check_launch("gated_activation_backward_kernel");
+int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float* gbu, const float* gy, const float* gate,
+                                     const float* up, int64_t nrow, int64_t ncol, int act, const float* hleaky, int acc,
+                                     hipStream_t stream) {
+    const bool wide = ncol % 4 == 0 && aligned16(ggate) && aligned16(gup) && aligned16(gy) && aligned16(gate) && aligned16(up);
+    const int64_t strip = wide ? 256 : 64, strips = (ncol + strip - 1) / strip;
+    // eight workgroups for a compute unit, and at least 16 rows for each
+    int64_t chunks = (8 * (int64_t)compute_units() + strips - 1) / strips;
+    if (chunks > (nrow + 15) / 16) chunks = (nrow + 15) / 16;
+    if (chunks > 65535) chunks = 65535;
+    const int64_t chunk = (nrow + chunks - 1) / chunks;
+    chunks = (nrow + chunk - 1) / chunk;
+    float* sums = nullptr;
+    // no scratch to be had (the stream is being captured and the buffer would have to grow): the sums read the gradients again
+    const bool wanted = gbg || gbu;
+    const bool fused = wanted && workspace(2 * chunks * ncol * (int64_t)sizeof(float), &sums) == KAI_OK;
+    if (!fused) {
+        sums = nullptr;
+        clear_error();
+    }
+    const dim3 grid((unsigned)strips, (unsigned)chunks);
+    if (wide) gated_activation_backward_kernel<4><<<grid, kThreads, 0, stream>>>(ggate, gup, sums, gy, gate, up, nrow, ncol, (int)chunk, act, hleaky);
+    else gated_activation_backward_kernel<1><<<grid, kThreads, 0, stream>>>(ggate, gup, sums, gy, gate, up, nrow, ncol, (int)chunk, act, hleaky);
+    KAI_TRY(check_launch("gated_activation_backward_kernel"));
+    if (!wanted) return KAI_OK;
+    if (!fused) {
+        if (gbg) KAI_TRY(launch_colsum(gbg, ggate, nrow, ncol, acc, stream));
+        return gbu ? launch_colsum(gbu, gup, nrow, ncol, acc, stream) : KAI_OK;
+    }
+    gated_bias_kernel<<<dim3((unsigned)((ncol + 63) / 64), 2), kThreads, 0, stream>>>(gbg, gbu, sums, ncol, (int)chunks, acc);
+    return check_launch("gated_bias_kernel");
 }
 
 int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
@@ -56,6 +143,7 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
     p.M = a.ndat; p.N = a.yvec; p.K = (int)a.xvec;
     p.lda = p.ldb = a.xvec; p.ldc = a.yvec;
     p.nwhich = 1;
+    if (gated_rows_pays(a)) return launch_gated_rows(a, stream);
     if (a.ndat > 32 && gated_gemm_applies(kGatedForward, p)) return launch_gated_gemm(kGatedForward, p, stream);
     // both products, then the activation and the product; the pre-activations in the caller's buffers or in scratch
     const int64_t n = a.ndat * a.yvec;

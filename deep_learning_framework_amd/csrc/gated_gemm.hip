@@ -38,7 +38,6 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 constexpr int kStep = 16;
 constexpr int kPadRows = 8;            // between the halves of a plane: the two halves' writes meet different banks
-constexpr float kBf16Limit = 3.38e38f; // above 3.3895e38 the first piece rounds to infinity
 
 __device__ __forceinline__ float* uniform_ptr(const float* p) {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
@@ -200,7 +199,7 @@ struct Shape {
 };
 
 template <int MODE, int WM, int WN, int NBM>
-__global__ __launch_bounds__(64 * WM * WN, NBM == 4 ? 2 : NBM == 2 ? 3 : 4) void gated_gemm_kernel(GatedGemm p) {
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) void gated_gemm_kernel(GatedGemm p) {
     using S = Shape<MODE, WM, WN, NBM>;
     using TA = typename S::TA;
     using TB = typename S::TB;
@@ -239,29 +238,29 @@ __global__ __launch_bounds__(64 * WM * WN, NBM == 4 ? 2 : NBM == 2 ? 3 : 4) void
     const int64_t bstart = S::BKC ? n0 * p.ldb : n0 + (kSegments == 1 ? (int64_t)s0 * kStep * p.ldb : 0);
     const int64_t aend = S::AKC ? (p.M - 1) * p.lda + p.K : (p.K - 1) * p.lda + p.M;
     const int64_t bend = S::BKC ? (p.N - 1) * p.ldb + p.K : (p.K - 1) * p.ldb + p.N;
-    __amdgpu_buffer_rsrc_t arsrc[kSegments], brsrc[2];
+    __amdgpu_buffer_rsrc_t arsrc[kSegments], brsrc[MODE == kGatedForward ? TB::kPieces : 2];
     // byte offsets of this thread's loads of step 0 from there
-    uint32_t aoff[2], boff[2];       // (a transposing thread's other loads are rows further on)
+    uint32_t aoff[TA::kPieces], boff[TB::kPieces];       // (a transposing thread's other loads are rows further on)
 #pragma unroll
     for (int g = 0; g < kSegments; g++) {
         const float* A = MODE == kGatedGw ? p.A[which] : p.A[g];
         arsrc[g] = rsrc_from(A + astart, A + aend);
     }
 #pragma unroll
-    for (int g = 0; g < 2; g++) {
+    for (int g = 0; g < (MODE == kGatedForward ? TB::kPieces : 2); g++) {
         // forward: rows of the tile alternate between the weights, 32 at a time, so a load's rows are of one of them
         const float* B = MODE == kGatedForward ? p.B[__builtin_amdgcn_readfirstlane(TB::row_of(g) / 32 % 2)] : p.B[g < kSegments ? g : 0];
         brsrc[g] = rsrc_from(B + bstart, B + bend);
     }
     if constexpr (S::AKC) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) aoff[i] = (uint32_t)(TA::row_of(i) * p.lda + TA::step_of()) * 4;
+        for (int i = 0; i < TA::kPieces; i++) aoff[i] = (uint32_t)(TA::row_of(i) * p.lda + TA::step_of()) * 4;
     } else {
         aoff[0] = (uint32_t)(TA::step_of() * p.lda + TA::row_of(0)) * 4;
     }
     if constexpr (S::BKC) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < TB::kPieces; i++)
             boff[i] = (uint32_t)((TB::row_of(i) % 32 + TB::row_of(i) / 64 * 32) * p.ldb + TB::step_of()) * 4;
     } else {
         boff[0] = (uint32_t)(TB::step_of() * p.ldb + TB::row_of(0)) * 4;
@@ -386,7 +385,7 @@ __global__ __launch_bounds__(64 * WM * WN, NBM == 4 ? 2 : NBM == 2 ? 3 : 4) void
 
     // Epilogue by way of LDS, a wave's own 32 rows at a time: the accumulators hold one column a lane, the stores want four
     // columns of a row, and the activation's code stands there once instead of once for every register.
-    const bool again = __syncthreads_or(!(largest < kBf16Limit));
+    const bool again = __syncthreads_or(!(largest <= kLargestFinite));
     const float leaky = MODE == kGatedForward && p.hleaky ? *p.hleaky : 0.0f;
     float* stage = reinterpret_cast<float*>(lds) + wave * S::kStageFloats;
     const int64_t n = n0 + wn * (MODE == kGatedForward ? 32 : 64) + lane % 8 * 4;      // this lane's columns,
@@ -526,27 +525,28 @@ int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
 }
 
 // The tile and the parts of the reduction that this estimate (us) finds cheapest.  A workgroup's step of 16 takes 0.42
-// (64 x 128 tiles), 0.70 (128 x 128) or 2.35 (256 x 256), the workgroups of a compute unit one after another (the small
-// tiles' run side by side, but share the matrix cores); its start and epilogue `fixed`; parts a launch of 4 and their sums
-// written and read at 10 bytes a ns.  Fitted to 35 shapes, 33 to 2048 rows by 64 to 4096 by 333 to 4096, against 1, 2, 3, 4, 6,
-// 8, 12 and 16 parts of each tile: within a tenth of the fastest for all but a few.  The sides, in us: 1000 x 777 -> 333 20.3 with two
-// parts of 64 x 128, 22.0 with four of 128 x 128; 512 x 1024 -> 4096 55 with 128 x 128, 58 with 64 x 128; 2048 x 1024 -> 4096 165 with
-// 256 x 256, 184 with 128 x 128; 256 x 4096 -> 4096 99 with eight parts of 256 x 256, 121 with 64 x 128 whole.
+// (64 x 128 tiles), 0.70 (128 x 128), 1.25 (256 x 128) or 2.35 (256 x 256), the workgroups of a compute unit one after another (the
+// small tiles' run side by side, but share the matrix cores); its start and epilogue `fixed`; parts a launch of 4 and their
+// sums written and read at 10 bytes a ns.  Fitted to 35 shapes, 33 to 2048 rows by 64 to 4096 by 333 to 4096, against 1, 2, 3, 4, 6, 8, 12
+// and 16 parts of each tile: within a tenth of the fastest for all but a few.  The sides, in us: 1000 x 777 -> 333 20.3 with two parts of
+// 64 x 128, 22.0 with four of 128 x 128; 1000 x 1024 -> 4096 90 with 256 x 128, 94 with 128 x 128; 2048 x 1024 -> 4096 161 with 256 x 256, 177 with
+// 256 x 128; 256 x 4096 -> 4096 96 with four parts of 256 x 128, 121 with 64 x 128 whole; the weights' gradients of 2048 x 1024 -> 4096
+// 200 with 256 x 128, 209 with two parts of 256 x 256, 210 with 128 x 128.
 struct Plan {
-    int tile = 0;      // 0: 64 x 128, 1: 128 x 128, 2: 256 x 256
+    int tile = 0;      // 0: 64 x 128, 1: 128 x 128, 2: 256 x 128, 3: 256 x 256
     int parts = 1;
     double us = 1e30;
 };
 
 template <int MODE>
 Plan plan_of(const GatedGemm& p) {
-    constexpr int rows[3] = {64, 128, 256}, columns[3] = {128, 128, 256};
-    constexpr double step[3] = {0.42, 0.70, 2.35};
-    constexpr double fixed_forward[3] = {7.7, 12.0, 19.0}, fixed_gradient[3] = {5.2, 6.5, 14.0};
+    constexpr int rows[4] = {64, 128, 256, 256}, columns[4] = {128, 128, 128, 256};
+    constexpr double step[4] = {0.42, 0.70, 1.25, 2.35};
+    constexpr double fixed_forward[4] = {7.7, 12.0, 15.0, 19.0}, fixed_gradient[4] = {5.2, 6.5, 8.0, 14.0};
     const int64_t all_columns = MODE == kGatedForward ? 2 * p.N : p.N, cu = compute_units();
     const int64_t steps = (p.K + kStep - 1) / kStep * (MODE == kGatedGx ? 2 : 1);
     Plan best;
-    for (int t = 0; t < 3; t++) {
+    for (int t = 0; t < 4; t++) {
         const int64_t tiles = (p.M + rows[t] - 1) / rows[t] * ((all_columns + columns[t] - 1) / columns[t]) * p.nwhich;
         for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
             if (parts > 1 && steps < 4 * parts) break;
@@ -564,6 +564,7 @@ int launch_mode(const GatedGemm& p, hipStream_t stream) {
     const Plan plan = plan_of<MODE>(p);
     if (plan.tile == 0) return launch_shape<MODE, 2, 2, 1>(p, plan.parts, stream);
     if (plan.tile == 1) return launch_shape<MODE, 2, 2, 2>(p, plan.parts, stream);
+    if (plan.tile == 2) return launch_shape<MODE, 4, 2, 2>(p, plan.parts, stream);
     return launch_shape<MODE, 2, 4, 4>(p, plan.parts, stream);
 }
 

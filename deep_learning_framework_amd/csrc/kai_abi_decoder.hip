@@ -204,11 +204,15 @@ int kai_gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* 
             held_bytes = 2 * n * (int64_t)sizeof(float);
             KAI_TRY(workspace(held_bytes, &work));
         }
-        KAI_TRY(launch_gated_activation_backward(work, work + n, pgy, pgate, pup, n, actFunc, hLeakyAlpha, current_stream()));
     }
     ScratchHold held(held_bytes);
-    if (pgbg) KAI_TRY(kai_add_bias_backward_b(device, pgbg, work, ndat, yvec, acc));
-    if (pgbu) KAI_TRY(kai_add_bias_backward_b(device, pgbu, n > 0 ? work + n : nullptr, ndat, yvec, acc));
+    if (n > 0) {
+        KAI_TRY(launch_gated_activation_backward(work, work + n, pgbg, pgbu, pgy, pgate, pup, ndat, yvec, actFunc, hLeakyAlpha,
+                                                 acc != 0, current_stream()));
+    } else {
+        if (pgbg) KAI_TRY(kai_add_bias_backward_b(device, pgbg, nullptr, ndat, yvec, acc));
+        if (pgbu) KAI_TRY(kai_add_bias_backward_b(device, pgbu, nullptr, ndat, yvec, acc));
+    }
     GatedGradArgs a{};
     a.gx = pgx; a.gwg = pgwg; a.gwu = pgwu;
     a.ggate = work; a.gup = n > 0 ? work + n : nullptr;

@@ -19,6 +19,8 @@ namespace kai {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 
+constexpr float kLargestFinite = 3.40282347e38f;
+
 struct Split8 {
     bf16x8 h, m, l;
 };
