@@ -629,6 +629,8 @@ int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
     while (nr > 1 && c.nbat * c.nkvhead * tiles_of_rows(nr) * most < 2 * cu) nr /= 2;
     const int64_t row_tiles = tiles_of_rows(nr);
     const int64_t groups = tiled ? c.nbat * c.nkvhead * row_tiles : (rows + 3) / 4;
+    // threads of a launch are counted in 32 bits
+    if (groups >= 1ll << 24) return fail(KAI_ERR_INVALID_ARGUMENT, "cache_attention: nbat * nkvhead above 2^23");
     const int64_t resident = nr == 4 ? 1 : 2;      // workgroups of a compute unit
     // One round of workgroups over the chip; two where sequences of different lengths may stand side by side and the parts
     // stay long (their workgroups then even out).  32 x 1 over 4096 to 1366 keys: one round 155 us, two 138; 1 x 16 over

@@ -107,6 +107,7 @@ int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float
                                      hipStream_t stream) {
     const bool wide = ncol % 4 == 0 && aligned16(ggate) && aligned16(gup) && aligned16(gy) && aligned16(gate) && aligned16(up);
     const int64_t strip = wide ? 256 : 64, strips = (ncol + strip - 1) / strip;
+    if (strips >= (1ll << 24)) return fail(KAI_ERR_INVALID_ARGUMENT, "gated_backward: too many columns");
     // eight workgroups for a compute unit, and at least 16 rows for each
     int64_t chunks = (8 * (int64_t)compute_units() + strips - 1) / strips;
     if (chunks > (nrow + 15) / 16) chunks = (nrow + 15) / 16;

@@ -570,9 +570,11 @@ int launch_mode(const GatedGemm& p, hipStream_t stream) {
 
 }  // namespace
 
-// Offsets inside a workgroup's operands are 32-bit: 256 rows of a K-contiguous operand, all steps of another.
+// Offsets inside a workgroup's operands are 32-bit (256 rows of a K-contiguous operand, all steps of another), and so are the
+// threads of a launch.
 bool gated_gemm_applies(int mode, const GatedGemm& p) {
     if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.lda >= (1ll << 21) || p.ldb >= (1ll << 21)) return false;
+    if ((p.M / 64 + 1) * (p.N / 64 + 1) >= (1ll << 22)) return false;
     const int64_t rows = (int64_t)p.K + kStep;
     if (mode != kGatedForward && rows * p.ldb >= (1ll << 30)) return false;
     return mode != kGatedGw || rows * p.lda < (1ll << 30);

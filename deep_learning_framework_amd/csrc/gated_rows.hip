@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_rows_kernel(GatedArgs a)
 // 17.2 | 9.4, 16 x 4096 -> 4096 29.0 | 27.1; 16 x 4096 -> 1024, where a quarter of the chip works, 20.6 | 24.2; 1 and 24 x 4096 -> 11008
 // 56.5 and 71.7 | 66.4 and 87.5, where it cuts the same x in 688 workgroups.
 bool gated_rows_pays(const GatedArgs& a) {
-    if (a.ndat > 32 || a.xvec <= 0 || a.xvec >= (1ll << 30)) return false;
+    if (a.ndat > 32 || a.xvec <= 0 || a.xvec >= (1ll << 30) || a.yvec >= (1ll << 26)) return false;   // 32-bit step and thread counts
     const double bytes = 8.0 * (double)a.xvec * (double)a.yvec, cu = compute_units();
     const double rounds = std::ceil((double)((a.yvec + 15) / 16) / cu);
     const double work = 3.5 + rounds * 2.0 * (double)a.xvec / 256.0 * (a.ndat <= 16 ? 0.47 : 0.62);

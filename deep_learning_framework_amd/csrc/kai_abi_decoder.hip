@@ -18,7 +18,7 @@ constexpr int64_t kMaxWidth = 1ll << 24;     // floats of a token's heads
 constexpr int64_t kMaxRotary = 512;          // rotated elements of a head
 constexpr int64_t kMaxAttentionPiece = 256;
 constexpr int64_t kMaxReach = 1ll << 30;           // keys of a sequence: indices a few tiles further on still fit 32 bits
-constexpr int64_t kMaxAttentionRows = 1ll << 26;   // a wave each: the threads of a launch stay below 2^32
+constexpr int64_t kMaxAttentionRows = 1ll << 25;   // a wave each: the threads of a launch stay below 2^32
 
 int rotary_params(const char* who, const kai_rotary_desc* desc, int64_t npiece, RotaryParams* out) {
     RotaryParams r{};
@@ -161,7 +161,7 @@ int kai_cache_attention(int device, float* py, const float* pQ, const float* pcK
     KAI_REQUIRE(npiece <= kMaxAttentionPiece, KAI_ERR_INVALID_ARGUMENT, "npiece above 256");
     if (nbat == 0 || ntimes == 0 || nhead == 0 || npiece == 0) return KAI_OK;
     KAI_REQUIRE(nkvhead > 0 && nhead % nkvhead == 0, KAI_ERR_INVALID_ARGUMENT, "nhead must be a multiple of nkvhead");
-    KAI_REQUIRE(nbat * ntimes <= kMaxAttentionRows / nhead, KAI_ERR_INVALID_ARGUMENT, "nbat * ntimes * nhead above 2^26");
+    KAI_REQUIRE(nbat * ntimes <= kMaxAttentionRows / nhead, KAI_ERR_INVALID_ARGUMENT, "nbat * ntimes * nhead above 2^25");
     KAI_REQUIRE_PTR(py); KAI_REQUIRE_PTR(pQ); KAI_REQUIRE_PTR(plen);
     if (npage > 0 && npagelen > 0 && nmaxpage > 0) { KAI_REQUIRE_PTR(pcK); KAI_REQUIRE_PTR(pcV); }
     KAI_REQUIRE(!overlap(py, nbat * ntimes * nhead * npiece * 4, pQ, ((nbat * ntimes - 1) * nvec + nhead * npiece) * 4),

@@ -452,9 +452,10 @@ int kai_cache_append(int device, float* pcK, float* pcV, const float* pK, const 
  * bits a row, in ceil(ntimes / 32) words), so that a drafted tree's node sees its ancestors and itself.  pmask null:
  * s <= t.  One new token is a step of plain decoding.  pQ is [nbat, ntimes, nvec] (head h at h * npiece, nhead * npiece <=
  * nvec), py[nbat, ntimes, nhead * npiece]; head h reads the keys of head h / (nhead / nkvhead) (nkvhead divides nhead).
- * npiece is at most 256.  A row that sees no key, or none whose score is above minus infinity, gives zeros; what
- * stands at keys that a row does not see (NaN included) does not reach it.  The keys are cut into parts whose
- * results meet in the library scratch. */
+ * npiece is at most 256, nbat * ntimes * nhead at most 2^25, nbat * nkvhead at most 2^23.  A row that sees no key, or none
+ * whose score is above minus infinity, gives zeros; what stands at keys that a row does not see (NaN included) does not
+ * reach it.  The keys are cut into parts whose results meet in the library scratch (nbat * ntimes * nhead * (npiece + 2)
+ * floats a part, up to 256 parts where there are few rows). */
 int kai_cache_attention(int device, float* py, const float* pQ, const float* pcK, const float* pcV, const int* ppage,
                         const int* plen, const int* pcount, const int* pmask, int64_t nbat, int64_t ntimes, int64_t nvec,
                         int64_t nhead, int64_t nkvhead, int64_t npiece, int64_t npage, int64_t npagelen, int64_t nmaxpage,

@@ -184,6 +184,8 @@ def test_cache_refusals():
     _refused(510, lambda: attend(nkv=3))
     _refused(510, lambda: attend(nkv=0))
     _refused(510, lambda: attend(npc=257, nvec=257 * 4))
+    _refused(510, lambda: attend(nbat=2 ** 22, nt=8))       # too many rows
+    _refused(510, lambda: attend(npage=2 ** 20, page=2 ** 12, most=1))
     _refused(523, lambda: attend(y=None))
     _refused(523, lambda: attend(q=None))
     _refused(510, lambda: attend(y=ONE, q=ONE))
@@ -498,6 +500,54 @@ def test_cache_attention_large_and_equal_scores():
     c = _attention_case(rng, 1, 4, 2, 1, 64, 16, [200], None, False)
     c["ck"] *= 1e-30
     _check_attention(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("npiece", [64, 20])
+def test_cache_attention_where_the_pages_run_out(npiece):
+    """New tokens that found no room are not seen, by themselves either; lengths behind the last page are cut."""
+    rng = np.random.default_rng(12)
+    c = _attention_case(rng, 3, 5, 4, 2, npiece, 16, [29, 32, 100], None, False)
+    c["most"], c["table"] = 2, np.ascontiguousarray(c["table"][:, :2])
+    _check_attention(c)
+    c["most"], c["table"] = 0, np.zeros((3, 1), np.int32)
+    assert np.all(_attend(c) == 0)
+
+
+@pytest.mark.gpu
+def test_cache_attention_many_rows_and_one_key_head():
+    rng = np.random.default_rng(13)
+    c = _attention_case(rng, 1, 257, 8, 1, 128, 64, [300], None, False)
+    _check_attention(c)
+
+
+@pytest.mark.gpu
+def test_cache_behind_four_gigabytes():
+    """Pages whose bytes lie behind 2^32: written and read where they are."""
+    rng = np.random.default_rng(14)
+    nkv, npiece, page, npage = 8, 128, 256, 5000                 # 5.2 GB each of keys and values
+    width = nkv * npiece
+    ck, cv = DeviceBuffer(npage * page * width * 4), DeviceBuffer(npage * page * width * 4)
+    table = dev_int([[4999, 3], [4500, 4998]])
+    d = kai.rotary_desc(128)
+    k, v = (rng.standard_normal((2, 300, width)).astype(np.float32) for _ in range(2))
+    lens = dev_int([0, 0])
+    VMath.cache_append(0, ck, cv, DeviceBuffer.from_numpy(k), DeviceBuffer.from_numpy(v), table, lens, None, None, 2, 300, width,
+                       nkv, npiece, npage, page, 2, d)
+    q = rng.standard_normal((2, 3, 16 * npiece)).astype(np.float32)
+    y = Tensor((2, 3, 16 * npiece))
+    lens, counts = dev_int([297, 200]), dev_int([3, 2])
+    VMath.cache_attention(0, y.ptr, DeviceBuffer.from_numpy(q), ck, cv, table, lens, counts, None, 2, 3, 16 * npiece, 16, nkv,
+                          npiece, npage, page, 2, kai.hyper(npiece ** -0.5))
+    got = y.numpy().reshape(2, 3, 16, npiece)
+    turned, _ = plain_rotary(k.reshape(2, 300, nkv, npiece), np.broadcast_to(np.arange(300), (2, 300)), d)
+    for b, (n, count) in enumerate(((297, 3), (200, 2))):
+        see = np.ones((count, n + count), bool)
+        see[:, n:] = np.tril(np.ones((count, count), bool))
+        want, room = plain_attention(q[b, :count].reshape(count, 16, npiece), turned[b, :n + count],
+                                     v[b, :n + count].reshape(-1, nkv, npiece), see, float(np.float32(npiece ** -0.5)))
+        # the keys' own rounding reaches the scores as another 10 half steps of a product's factor
+        assert np.all(np.abs(got[b, :count] - want) <= 8 * room)
 
 
 @pytest.mark.gpu
