@@ -86,8 +86,9 @@ __device__ void turn_unit(float* y, const float* x, const float2* cs, int u, int
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         const float2 t = cs[i0 + e];
-        ya[e] = a[e] * t.x - b[e] * t.y;
-        yb[e] = b[e] * t.x + a[e] * t.y;
+        // which product the sum keeps unrounded is written out: the same bits whatever the vectors' width
+        ya[e] = fmaf(a[e], t.x, -(b[e] * t.y));
+        yb[e] = fmaf(b[e], t.x, a[e] * t.y);
     }
     vec w1, w2;
 #pragma unroll

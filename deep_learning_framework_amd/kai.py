@@ -108,6 +108,10 @@ class RotaryDesc(ctypes.Structure):
     _fields_ = [("nrot", ctypes.c_int64), ("layout", ctypes.c_int32), ("scaling", ctypes.c_int32)] + [
         (n, ctypes.c_double) for n in ("base", "factor", "trained", "low_turns", "high_turns", "magnitude")]
 
+    @property
+    def _as_parameter_(self):
+        return ctypes.addressof(self)
+
 
 def rotary_desc(nrot, layout="halves", base=10000.0, scaling="none", factor=1.0, trained=0.0, low_turns=1.0,
                 high_turns=4.0, magnitude=1.0):
@@ -163,10 +167,6 @@ def _addr(p):
     return int(p)
 
 
-def _desc(desc):
-    return None if desc is None else ctypes.addressof(desc)
-
-
 class DeviceBuffer:
     """Device memory owned through VMath::mem_alloc / mem_free semantics (kai_mem_alloc)."""
 
@@ -190,6 +190,11 @@ class DeviceBuffer:
         if out.nbytes:
             _ck(load().kai_memcpy_to_host(self.device, out.ctypes.data, self.ptr, out.nbytes))
         return out
+
+    @property
+    def _as_parameter_(self):
+        """The address, where ctypes is given the buffer itself."""
+        return self.ptr
 
     def offset(self, nbytes):
         """Raw address inside the buffer (sub-buffer pointers, as the engine's RNN driver passes)."""
@@ -493,42 +498,52 @@ class VMath:
                                       _addr(pw), _addr(px), _addr(ppre), yvec, ndat, xvec, actFunc,
                                       _addr(hLeakyAlpha), int(acc)))
 
-    # a decoder block: rotary positions, the cache of keys and values, the gated feed-forward projection
+    # A decoder block: rotary positions, the cache of keys and values, the gated feed-forward projection.  The calls of a
+    # decoding step take some microseconds each, so these pass their arguments on as they are (addresses, buffers by
+    # their _as_parameter_) and look no further than the status.
     @staticmethod
     def rotary(device, py, px, ppos, nbat, ntimes, nvec, nhead, npiece, desc):
         """Turn the heads of px by their tokens' positions; ``desc`` is a ``rotary_desc(...)``."""
-        _ck(load().kai_rotary(device, _addr(py), _addr(px), _addr(ppos), nbat, ntimes, nvec, nhead, npiece, _desc(desc)))
+        rc = (_lib or load()).kai_rotary(device, py, px, ppos, nbat, ntimes, nvec, nhead, npiece, desc)
+        if rc:
+            _ck(rc)
 
     @staticmethod
     def rotary_backward(device, pgx, pgy, ppos, nbat, ntimes, nvec, nhead, npiece, desc):
-        _ck(load().kai_rotary_backward(device, _addr(pgx), _addr(pgy), _addr(ppos), nbat, ntimes, nvec, nhead, npiece,
-                                       _desc(desc)))
+        rc = (_lib or load()).kai_rotary_backward(device, pgx, pgy, ppos, nbat, ntimes, nvec, nhead, npiece, desc)
+        if rc:
+            _ck(rc)
 
     @staticmethod
     def cache_append(device, pcK, pcV, pK, pV, ppage, plen, pcount, ppos, nbat, ntimes, nvec, nkvhead, npiece, npage,
                      npagelen, nmaxpage, desc):
         """Write new keys (turned by ``desc``, None: as they are) and values behind those of the cache."""
-        _ck(load().kai_cache_append(device, _addr(pcK), _addr(pcV), _addr(pK), _addr(pV), _addr(ppage), _addr(plen),
-                                    _addr(pcount), _addr(ppos), nbat, ntimes, nvec, nkvhead, npiece, npage, npagelen,
-                                    nmaxpage, _desc(desc)))
+        rc = (_lib or load()).kai_cache_append(device, pcK, pcV, pK, pV, ppage, plen, pcount, ppos, nbat, ntimes, nvec,
+                                               nkvhead, npiece, npage, npagelen, nmaxpage, desc)
+        if rc:
+            _ck(rc)
 
     @staticmethod
     def cache_attention(device, py, pQ, pcK, pcV, ppage, plen, pcount, pmask, nbat, ntimes, nvec, nhead, nkvhead, npiece,
                         npage, npagelen, nmaxpage, hCoef):
         """Attention of new tokens (a drafted tree with visibility words ``pmask``, or a run of tokens) over the cache."""
-        _ck(load().kai_cache_attention(device, _addr(py), _addr(pQ), _addr(pcK), _addr(pcV), _addr(ppage), _addr(plen),
-                                       _addr(pcount), _addr(pmask), nbat, ntimes, nvec, nhead, nkvhead, npiece, npage,
-                                       npagelen, nmaxpage, _addr(hCoef)))
+        rc = (_lib or load()).kai_cache_attention(device, py, pQ, pcK, pcV, ppage, plen, pcount, pmask, nbat, ntimes, nvec,
+                                                  nhead, nkvhead, npiece, npage, npagelen, nmaxpage, hCoef)
+        if rc:
+            _ck(rc)
 
     @staticmethod
     def gated_forward(device, py, pgate, pup, pwg, pwu, pbg, pbu, px, yvec, ndat, xvec, actFunc, hLeakyAlpha):
         """py = act(px . pwg^T + pbg) * (px . pwu^T + pbu)."""
-        _ck(load().kai_gated_forward(device, _addr(py), _addr(pgate), _addr(pup), _addr(pwg), _addr(pwu), _addr(pbg),
-                                     _addr(pbu), _addr(px), yvec, ndat, xvec, actFunc, _addr(hLeakyAlpha)))
+        rc = (_lib or load()).kai_gated_forward(device, py, pgate, pup, pwg, pwu, pbg, pbu, px, yvec, ndat, xvec, actFunc,
+                                                hLeakyAlpha)
+        if rc:
+            _ck(rc)
 
     @staticmethod
     def gated_backward(device, pgx, pgwg, pgwu, pgbg, pgbu, pga_work, pgy, pwg, pwu, px, pgate, pup, yvec, ndat, xvec,
                        actFunc, hLeakyAlpha, acc):
-        _ck(load().kai_gated_backward(device, _addr(pgx), _addr(pgwg), _addr(pgwu), _addr(pgbg), _addr(pgbu),
-                                      _addr(pga_work), _addr(pgy), _addr(pwg), _addr(pwu), _addr(px), _addr(pgate),
-                                      _addr(pup), yvec, ndat, xvec, actFunc, _addr(hLeakyAlpha), int(acc)))
+        rc = (_lib or load()).kai_gated_backward(device, pgx, pgwg, pgwu, pgbg, pgbu, pga_work, pgy, pwg, pwu, px, pgate, pup,
+                                                 yvec, ndat, xvec, actFunc, hLeakyAlpha, acc)
+        if rc:
+            _ck(rc)
