@@ -540,8 +540,8 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentio
     if (lane == 0) scratch[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
-    // a part that saw no key has a sum of 0
-    const float mine = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : expf(ml.x - top);
+    // a part that saw no key has a sum of 0; one whose scores are all NaN has a NaN, and no maximum that weighs it
+    const float mine = ml.y == 0.0f ? 0.0f : ml.y != ml.y ? ml.y : ml.x == top ? 1.0f : expf(ml.x - top);
     weight[threadIdx.x] = mine;
     float sum = mine == 0.0f ? 0.0f : mine * ml.y;
 #pragma unroll
@@ -558,7 +558,8 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentio
         for (int i = 0; i < kMaxPiece / kWave; i++) {
             const int d = lane + i * kWave;
             const float v = d < c.npiece ? from[d] : 0.0f;
-            if (w != 0.0f) acc[i] += w * v;
+            // a weight that has vanished takes a sum that passed the largest float away, but no NaN
+            if (w != 0.0f || v != v) acc[i] += w * v;
         }
     }
 #pragma unroll

@@ -118,7 +118,7 @@ int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float
     // no scratch to be had (the stream is being captured and the buffer would have to grow): the sums read the gradients again
     const bool wanted = gbg || gbu;
     const bool fused = wanted && workspace(2 * chunks * ncol * (int64_t)sizeof(float), &sums) == KAI_OK;
-    if (!fused) {
+    if (wanted && !fused) {
         sums = nullptr;
         clear_error();
     }

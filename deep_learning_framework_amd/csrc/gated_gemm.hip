@@ -12,8 +12,8 @@
 // consecutive rows, read and (but for K-contiguous operands' half chunks) written without bank conflicts.
 //
 // What lies outside an operand reads as 0 (buffer loads end with it); the last, partial step of a K-contiguous operand is
-// masked.  Where an operand held an infinity, or a value that rounds to one in bf16, sums that came out as NaN are formed
-// again in plain fp32, so that an infinity has the effect it has there.
+// masked.  Where an operand held an infinity, which the pieces turn into a NaN, sums that came out as NaN are formed again in
+// plain fp32, so that an infinity has the effect it has there.
 #include <type_traits>
 
 #include "act_funcs.h"

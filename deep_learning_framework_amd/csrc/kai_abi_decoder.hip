@@ -108,7 +108,8 @@ int cache_pages(const char* who, CachePages* c, const int* ppage, const int* ple
     if (ppage == nullptr && (nmaxpage > 1 || npage < nbat))
         return fail(KAI_ERR_INVALID_ARGUMENT, name + ": without a page table each sequence has one page, its own");
     c->table = ppage; c->len = plen; c->count = pcount;
-    c->nbat = nbat; c->ntimes = ntimes; c->npage = npage; c->page = npagelen; c->nmaxpage = nmaxpage;
+    // no page, no key: a kernel reads row 0 in place of a key that does not exist, so one must be there where keys are
+    c->nbat = nbat; c->ntimes = ntimes; c->npage = npage; c->page = npagelen; c->nmaxpage = npage > 0 ? nmaxpage : 0;
     c->nkvhead = (int)nkvhead; c->npiece = (int)npiece;
     return KAI_OK;
 }

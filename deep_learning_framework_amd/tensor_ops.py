@@ -453,7 +453,7 @@ def gated(x, wg, wu, bg=None, bu=None, actfunc="swish", leaky_alpha=None, keep=F
         if b is not None and b.total_size() != wg.shape[0]:
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "gated")
     yvec, xvec = wg.shape
-    ndat = x.total_size() // xvec
+    ndat = _total(x.shape[:-1])
     code = ACT[actfunc] if isinstance(actfunc, str) else int(actfunc)
     h = kai.hyper(leaky_alpha, x.device)
     y = Tensor(x.shape[:-1] + (yvec,), x.device)
@@ -471,7 +471,7 @@ def gated_backprop(y, ygrad):
     """The gradients of ``gated`` by name: x, wg, wu and, where there are biases, bg and bu."""
     s = y.saved
     yvec, xvec = s["wg"].shape
-    ndat = s["x"].total_size() // xvec
+    ndat = _total(s["x"].shape[:-1])
     dev = y.device
     g = {name: Tensor(s[name].shape, dev) for name in ("x", "wg", "wu", "bg", "bu") if s[name] is not None}
     ptr = lambda name: g[name].ptr if name in g else None
@@ -501,12 +501,15 @@ class KeyValueCache:
         self._len = DeviceBuffer.from_numpy(self.lengths, device)
 
     def accept(self, counts):
-        """Each sequence is ``counts`` (a number, or one per sequence) tokens longer."""
+        """Each sequence is ``counts`` (a number, or one per sequence) tokens longer.  The lengths change where they stand,
+        for recorded graphs name the place, and behind all that still reads them."""
         longer = self.lengths + np.asarray(counts, np.int32)
-        if np.any(longer < 0) or np.any(longer > self.npagelen * self.nmaxpage):
+        if longer.shape != (self.nbat,) or np.any(longer < 0) or np.any(longer > self.npagelen * self.nmaxpage):
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "accept")
+        kai.synchronize()
         self.lengths = longer.astype(np.int32)
-        self._len = DeviceBuffer.from_numpy(self.lengths, self.device)
+        if self.nbat:
+            kai._ck(kai.load().kai_memcpy_from_host(self.device, self._len.ptr, self.lengths.ctypes.data, self.lengths.nbytes))
 
     def append(self, key, value, counts=None, positions=None):
         if len(key.shape) != 3 or key.shape != value.shape or key.shape[0] != self.nbat or \

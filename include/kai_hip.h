@@ -79,7 +79,8 @@ int kai_device_synchronize(void);
 int kai_set_stream(void* hip_stream);
 /* Releases the scratch memory the library allocated for itself (partial sums of reductions cut into parts,
  * of the column sums of long narrow matrices, row norms of kai_cosinesim, the probabilities of a kai_attention_forward call that runs as separate
- * kernels; one buffer per device, created on first need).  Waits for the device first.  The library stays
+ * kernels, the parts of kai_cache_attention, the gradients in front of a kai_gated_backward without a work buffer, the
+ * sums of a kai_gated_forward that runs as separate kernels; one buffer per device, created on first need).  Waits for the device first.  The library stays
  * usable: the buffer is created again on demand.  No counterpart in the reference, whose kernels need no
  * scratch. */
 int kai_shutdown(void);
@@ -87,7 +88,9 @@ int kai_shutdown(void);
  * nothing: for callers that record calls into a HIP graph (a call whose scratch would have to grow while its
  * stream is being captured fails with KAI_ERR_GPU) or that cannot tolerate an allocation inside a step.  A
  * product never asks for more than 64 MiB of partial sums; kai_attention_forward outside the fused head sizes
- * asks for nbat*ntimes*ntimes*nhead floats on top.  Growing never waits for the device: the smaller buffer is
+ * asks for nbat*ntimes*ntimes*nhead floats on top; kai_cache_attention for what its declaration says;
+ * kai_gated_backward without a work buffer for 2*ndat*yvec floats, kai_gated_forward with null pgate at most for as many,
+ * and either for up to 16 parts of its products' results.  Growing never waits for the device: the smaller buffer is
  * kept until kai_shutdown, so work in flight and recorded graphs stay valid.  No counterpart in the reference. */
 int kai_reserve_scratch(int64_t bytes);
 /* Current size of the current device's scratch, how many times it was allocated or grown since the last
@@ -435,7 +438,7 @@ int kai_rotary_backward(int device, float* pgx, const float* pgy, const int* ppo
  * outside [0, npage) names no page: writes to it are dropped, its keys are not seen; nor are keys at nmaxpage *
  * npagelen and behind (at most 2^30; npage * npagelen is below 2^31).  plen[nbat] is the number of keys a sequence holds already (negative: 0); the new
  * ones stand behind it.  pcount[nbat], or null for ntimes, is how many of the ntimes rows of a sequence are new tokens
- * (clipped to 0 .. ntimes): the rows behind it are not read, and their results are left as they were. */
+ * (clipped to 0 .. ntimes): what stands in the rows behind it does not matter, and their results are left as they were. */
 
 /* Writes the keys pK and values pV[nbat, ntimes, nvec] (head h at h * npiece, nkvhead * npiece <= nvec) of the new tokens
  * behind the sequences' own, the keys turned on the way as kai_rotary does (desc null: not turned) by the positions
