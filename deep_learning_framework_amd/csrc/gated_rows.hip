@@ -130,18 +130,21 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_rows_kernel(GatedArgs a)
 
 }  // namespace
 
-// Against two of the dense layer's products and the activation behind them (about 9.3 us and the weights at 6300 bytes a ns):
-// this kernel's waves, two a SIMD and round of workgroups, take 0.47 us (16 rows) or 0.62 for each 256 of the reduction, and
-// the weights come at 5700 or 4300 bytes a ns.  Measured (us, two products | this kernel): 24 x 256 -> 512 9.3 | 5.0, 16 x 1024 -> 4096
-// 17.2 | 9.4, 16 x 4096 -> 4096 29.0 | 27.1; 16 x 4096 -> 1024, where a quarter of the chip works, 20.6 | 24.2; 1 and 24 x 4096 -> 11008
-// 56.5 and 71.7 | 66.4 and 87.5, where it cuts the same x in 688 workgroups.
+// Against two of the dense layer's products and the activation behind them.  Both sides as straight lines through 55
+// measurements (1, 4, 16, 24 and 32 rows of 11 shapes, weights from HBM): this kernel takes its waves' chain of steps, one in
+// flight at a time, or the weights at 5900 bytes a ns and less with more rows (every workgroup cuts the same x); the products
+// take three launches and the weights at 7000 or 6000.  Measured (us, two products | this kernel): 24 x 256 -> 512 8.8 | 5.0,
+// 16 x 1024 -> 4096 17.6 | 10.1, 16 and 32 x 4096 -> 4096 29.2 and 37.0 | 26.7 and 33.7, 1 x the same 24.7 | 25.4;
+// 16 x 4096 -> 1024, where a quarter of the chip works, 20.7 | 24.5; 1, 16 and 24 x 4096 -> 11008 57.9, 63.5 and
+// 72.1 | 64.2, 74.0 and 87.0.
 bool gated_rows_pays(const GatedArgs& a) {
     if (a.ndat > 32 || a.xvec <= 0 || a.xvec >= (1ll << 30) || a.yvec >= (1ll << 26)) return false;   // 32-bit step and thread counts
-    const double bytes = 8.0 * (double)a.xvec * (double)a.yvec, cu = compute_units();
-    const double rounds = std::ceil((double)((a.yvec + 15) / 16) / cu);
-    const double work = 3.5 + rounds * 2.0 * (double)a.xvec / 256.0 * (a.ndat <= 16 ? 0.47 : 0.62);
-    const double read = 3.0 + bytes / (a.ndat <= 16 ? 5.7e6 : 4.3e6);
-    return (work > read ? work : read) < 9.3 + bytes / 6.3e6;
+    const double bytes = 8.0 * (double)a.xvec * (double)a.yvec, rows = (double)a.ndat;
+    const double rounds = std::ceil((double)((a.yvec + 15) / 16) / (2.0 * compute_units()));
+    const double work = 3.2 + rounds * (double)a.xvec / 256.0 * (0.93 + 0.0265 * rows);
+    const double read = 3.2 + bytes / (5.9e6 - 0.05e6 * rows);
+    const double products = (a.ndat == 1 ? 6.5 : 8.5 + 0.17 * rows) + bytes / (a.ndat <= 16 ? 7.0e6 : 6.0e6);
+    return (work > read ? work : read) < products;
 }
 
 int launch_gated_rows(const GatedArgs& a, hipStream_t stream) {

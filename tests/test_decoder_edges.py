@@ -7,7 +7,7 @@ from deep_learning_framework_amd import kai
 from deep_learning_framework_amd.kai import DeviceBuffer, KaiError, VMath
 from deep_learning_framework_amd.tensor_ops import KeyValueCache, Tensor, gated, gated_backprop
 
-from test_decoder_ops import _attend, _attention_case, _expected, dev_int
+from test_decoder_ops import ACTS, REL_FRO_TOL, _attend, _attention_case, _expected, dev_int, rel_fro
 
 
 @pytest.mark.gpu
@@ -70,3 +70,20 @@ def test_accepted_lengths_stand_where_they_stood():
         with pytest.raises((KaiError, ValueError)):
             cache.accept(counts)
     assert np.array_equal(cache._len.to_numpy(2, np.int32), [5, 3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat,xvec,yvec", [(2, 4096, 260), (24, 4096, 260), (32, 4096, 97), (32, 512, 1030), (16, 1025, 2049)])
+def test_gated_few_rows_both_ways(ndat, xvec, yvec):
+    """Up to 32 rows: long reductions with few outputs run as the dense layer's products, the others in one launch."""
+    rng = np.random.default_rng(ndat + yvec)
+    x = rng.standard_normal((ndat, xvec)).astype(np.float32)
+    wg, wu = ((rng.uniform(-1, 1, (yvec, xvec)) * xvec ** -0.5).astype(np.float32) for _ in range(2))
+    bu = rng.standard_normal(yvec).astype(np.float32)
+    T = Tensor.from_numpy
+    y = gated(T(x), T(wg), T(wu), None, T(bu), actfunc="swish", keep=True)
+    gate, up = x.astype(np.float64) @ wg.T, x.astype(np.float64) @ wu.T + bu
+    assert rel_fro(y.saved["gate"].numpy(), gate) <= REL_FRO_TOL
+    assert rel_fro(y.saved["up"].numpy(), up) <= REL_FRO_TOL
+    assert rel_fro(y.numpy(), ACTS["swish"][0](gate) * up) <= REL_FRO_TOL
+    assert np.array_equal(gated(T(x), T(wg), T(wu), None, T(bu), actfunc="swish").numpy(), y.numpy())
