@@ -623,11 +623,15 @@ int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
     const bool tiled = tiled_applies(a);
     const int64_t shared_rows = c.ntimes * (a.nhead / c.nkvhead);      // of a key head
     const int64_t cu = compute_units();
-    const int64_t most = reach / 128 < 1 ? 1 : reach / 128 > kMaxParts ? kMaxParts : reach / 128;   // a tile for each wave
-    // The largest tile of rows that the rows fill and that leaves two workgroups for a compute unit
+    // parts down to a tile of 32 keys for each wave
+    const int64_t tiles = (reach + 127) / 128, most = tiles < 1 ? 1 : tiles > kMaxParts ? kMaxParts : tiles;
+    // The largest tile of rows that the rows fill: each tile cuts the same keys and values into pieces.  64 rows where that leaves
+    // two workgroups for a compute unit, 32 where it leaves half a one (32 heads of 128 on 8 key heads, 16 tokens over 4000 keys:
+    // 64 rows, 256 workgroups 27.3 us, 32 rows 23.8; over 2000 32 rows, 256 workgroups 18.0, 16 rows 21.5; 8 over 1000 32 rows, 64
+    // workgroups 15.7, 16 rows 14.3).
     int nr = shared_rows <= 16 ? 1 : shared_rows <= 32 ? 2 : 4;
     const auto tiles_of_rows = [&](int n) { return (shared_rows + 16 * n - 1) / (16 * n); };
-    while (nr > 1 && c.nbat * c.nkvhead * tiles_of_rows(nr) * most < 2 * cu) nr /= 2;
+    while (nr > 1 && c.nbat * c.nkvhead * tiles_of_rows(nr) * most < (nr == 4 ? 2 * cu : cu / 2)) nr /= 2;
     const int64_t row_tiles = tiles_of_rows(nr);
     const int64_t groups = tiled ? c.nbat * c.nkvhead * row_tiles : (rows + 3) / 4;
     // threads of a launch are counted in 32 bits
