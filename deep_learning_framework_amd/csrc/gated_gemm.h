@@ -20,9 +20,9 @@ struct GatedGemm {
     int nwhich;             // gw: 2 products, or 1; otherwise 1
     // filled by the launcher
     int tiles_m, tiles_n, run, part_steps;
-    int64_t ldp;            // row length of a part's sums
+    int whole, cut, nparts; // tiles that one workgroup takes whole; the others, and the parts of the reduction of each
     int wide;               // outputs in rows of whole 16-byte lines
-    float* parts;           // partial sums of a reduction cut into parts; null: whole
+    float* parts;           // [nparts][cut] tiles of sums
 };
 
 bool gated_gemm_applies(int mode, const GatedGemm& p);

@@ -12,8 +12,8 @@
 // consecutive rows, read and (but for K-contiguous operands' half chunks) written without bank conflicts.
 //
 // Bound: the matrix cores at a sixth of their bf16 rate (235 TFLOP/s of fp32 products at what large bf16 products reach, 1412),
-// with the cutting's vector instructions between them.  4096 x 4096 -> 11008 forward 3.38 ms = 219 TFLOP/s; gradients of 2048 x 1024 ->
-// 4096 177 and 178 us = 194 and 193 TFLOP/s; small products the chain of their steps (1000 x 777 -> 333 16.7 us and 4.9 for the
+// with the cutting's vector instructions between them.  4096 x 4096 -> 11008 forward 3.19 ms = 232 TFLOP/s; gradients of 2048 x 1024 ->
+// 4096 177 and 178 us = 194 and 193 TFLOP/s; small products the chain of their steps (1000 x 777 -> 333 17 us and 5.4 for the
 // sums of two parts).
 //
 // What lies outside an operand reads as 0 (buffer loads end with it); the last, partial step of a K-contiguous operand is
@@ -203,6 +203,26 @@ struct Shape {
     static constexpr int kColumns = MODE == kGatedForward ? BN / 2 : BN;    // of the output that a tile covers
 };
 
+// Neighbouring tiles on one XCD (workgroup ids go round the eight).
+__device__ __forceinline__ int on_one_xcd(int id, int total) {
+    const int each = total / 8, rest = total % 8, xcd = id % 8, at = id / 8;
+    return xcd * each + (xcd < rest ? xcd : rest) + at;
+}
+
+struct Place {
+    int which, tm, tn;
+};
+// Tiles in runs of `run` tile rows by all columns
+__device__ __forceinline__ Place place_of(const GatedGemm& p, int id) {
+    const int tiles_mn = p.tiles_m * p.tiles_n, which = id / tiles_mn;
+    id -= which * tiles_mn;
+    const int run = p.run * p.tiles_n;
+    const int first = id / run * p.run;
+    const int rows = p.tiles_m - first < p.run ? p.tiles_m - first : p.run;
+    const int in = id % run;
+    return Place{which, first + in % rows, in / rows};
+}
+
 template <int MODE, int WM, int WN, int NBM>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) void gated_gemm_kernel(GatedGemm p) {
     using S = Shape<MODE, WM, WN, NBM>;
@@ -213,29 +233,18 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int wm = wave / WN, wn = wave % WN;
 
-    // Tiles in runs of `run` tile rows by all columns, and consecutive ones on one XCD (workgroup ids go round the eight)
-    int tm, tn, which;
-    {
-        const int tiles_mn = p.tiles_m * p.tiles_n, total = tiles_mn * p.nwhich;
-        int id = blockIdx.x;
-        const int each = total / 8, rest = total % 8, xcd = id % 8, at = id / 8;
-        id = xcd * each + (xcd < rest ? xcd : rest) + at;
-        which = id / tiles_mn;
-        id -= which * tiles_mn;
-        const int run = p.run * p.tiles_n;
-        const int first = id / run * p.run;
-        const int rows = p.tiles_m - first < p.run ? p.tiles_m - first : p.run;
-        const int in = id % run;
-        tm = first + in % rows;
-        tn = in / rows;
-    }
-    const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * S::kColumns;
+    // The first p.whole workgroups take a tile each, those behind them a part of the reduction of one of the p.cut others.
+    const bool partial = (int)blockIdx.x >= p.whole;
+    const int behind = (int)blockIdx.x - p.whole, part = partial ? behind / p.cut : 0, cut = partial ? behind % p.cut : 0;
+    const Place place = partial ? place_of(p, p.whole + on_one_xcd(cut, p.cut)) : place_of(p, on_one_xcd((int)blockIdx.x, p.whole));
+    const int which = place.which;
+    const int64_t m0 = (int64_t)place.tm * S::BM, n0 = (int64_t)place.tn * S::kColumns;
     // Whole steps [s0, s1) of this part of the reduction; the last part takes the rests (K % 16 steps a segment) as well.
     constexpr int kSegments = MODE == kGatedGx ? 2 : 1;
     const int full = p.K / kStep;
-    const int s0 = (int)blockIdx.y * p.part_steps;
-    const int s1 = s0 + p.part_steps < kSegments * full ? s0 + p.part_steps : kSegments * full;
-    const bool rests = blockIdx.y + 1 == gridDim.y && p.K % kStep != 0;
+    const int s0 = part * p.part_steps;
+    const int s1 = partial && s0 + p.part_steps < kSegments * full ? s0 + p.part_steps : kSegments * full;
+    const bool rests = (!partial || part + 1 == p.nparts) && p.K % kStep != 0;
 
     // Buffers that end with the operands.  K-contiguous operands start at the tile's first row, the others at its first
     // column and, with one segment, at the part's first step: offsets inside stay below 4 GiB.
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) 
     const int64_t n = n0 + wn * (MODE == kGatedForward ? 32 : 64) + lane % 8 * 4;      // this lane's columns,
     const int64_t n2 = MODE == kGatedForward ? n : n + 32;                           // and the other block's
     f32x4 bg, bu;
-    if (MODE == kGatedForward && p.parts == nullptr) {
+    if (MODE == kGatedForward && !partial) {
         bg = bias4(p.bias[0], n, p.N);
         bu = bias4(p.bias[1], n, p.N);
     }
@@ -427,25 +436,21 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) 
             const float* row = stage + r * kStageRow + lane % 8 * 4;
             f32x4 v = *reinterpret_cast<const f32x4*>(row), u = *reinterpret_cast<const f32x4*>(row + 32);
             const int64_t at = m * p.ldc;
-            if constexpr (MODE == kGatedForward) {
-                if (p.parts) {
-                    float* part = p.parts + ((int64_t)blockIdx.y * 2 * p.M + m) * p.ldp;
-                    put(part, n, p.ldp, v, 1);
-                    put(part + p.M * p.ldp, n, p.ldp, u, 1);
-                } else {
-                    v += bg;
-                    u += bu;
-                    const f32x4 y = activate4(v, p.act, leaky) * u;
-                    if (p.C[1]) {
-                        put(p.C[1] + at, n, p.N, v, p.wide);
-                        put(p.C[2] + at, n, p.N, u, p.wide);
-                    }
-                    put(p.C[0] + at, n, p.N, y, p.wide);
+            if (partial) {
+                // the tile as it stands, a wave's two blocks of 32 columns side by side
+                f32x4* sums = reinterpret_cast<f32x4*>(p.parts) +
+                              (((int64_t)part * p.cut + cut) * S::BM + (m - m0)) * (S::BN / 4) + wn * 16 + lane % 8;
+                sums[0] = v;
+                sums[8] = u;
+            } else if constexpr (MODE == kGatedForward) {
+                v += bg;
+                u += bu;
+                const f32x4 y = activate4(v, p.act, leaky) * u;
+                if (p.C[1]) {
+                    put(p.C[1] + at, n, p.N, v, p.wide);
+                    put(p.C[2] + at, n, p.N, u, p.wide);
                 }
-            } else if (p.parts) {
-                float* part = p.parts + (((int64_t)blockIdx.y * p.nwhich + which) * p.M + m) * p.ldp;
-                put(part, n, p.ldp, v, 1);
-                put(part, n2, p.ldp, u, 1);
+                put(p.C[0] + at, n, p.N, y, p.wide);
             } else {
                 float* c0 = p.C[which] + at;
                 if (p.acc) {
@@ -462,44 +467,51 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : NBM == 2 ? 3 : 4) 
     }
 }
 
-// Sums the parts (rows of whole 16-byte lines, four columns a thread), with the forward's epilogue or onto the gradient.
-template <int MODE>
-__global__ __launch_bounds__(256) void gated_parts_kernel(GatedGemm p, int nparts) {
-    const int lines = (int)(p.ldp / 4);
-    const int64_t one = p.M * lines, total = one * (MODE == kGatedForward ? 1 : p.nwhich);
-    const int64_t all = one * (MODE == kGatedForward ? 2 : p.nwhich);
+// Sums the parts of the tiles that were cut, with the forward's epilogue or onto the gradient: a thread takes four columns of a
+// row and, for the forward, the same four of gate and of up.
+template <int MODE, int BM, int BN>
+__global__ __launch_bounds__(256) void gated_parts_kernel(GatedGemm p) {
+    constexpr int kLines = (MODE == kGatedForward ? BN / 2 : BN) / 4;      // of an output row that a tile covers
+    constexpr int kGroups = BM * kLines / 256;                             // workgroups of a tile
+    const int64_t all = (int64_t)p.cut * BM * (BN / 4);
     const float leaky = MODE == kGatedForward && p.hleaky ? *p.hleaky : 0.0f;
     const f32x4* parts = reinterpret_cast<const f32x4*>(p.parts);
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        f32x4 v = parts[e], u = MODE == kGatedForward ? parts[one + e] : v;
+    const int cut = (int)blockIdx.x / kGroups, e = (int)blockIdx.x % kGroups * 256 + (int)threadIdx.x;
+    const int line = e % kLines, row = e / kLines;
+    const Place place = place_of(p, p.whole + on_one_xcd(cut, p.cut));
+    const int64_t m = (int64_t)place.tm * BM + row, n = ((int64_t)place.tn * kLines + line) * 4;
+    if (m >= p.M || n >= p.N) return;
+    const f32x4* from = parts + ((int64_t)cut * BM + row) * (BN / 4) + (MODE == kGatedForward ? line / 8 * 16 + line % 8 : line);
+    f32x4 v = from[0], u = MODE == kGatedForward ? from[8] : v;
 #pragma unroll 4
-        for (int s = 1; s < nparts; s++) {
-            v += parts[s * all + e];
-            if (MODE == kGatedForward) u += parts[s * all + one + e];
+    for (int s = 1; s < p.nparts; s++) {
+        v += from[s * all];
+        if (MODE == kGatedForward) u += from[s * all + 8];
+    }
+    const int64_t at = m * p.ldc;
+    if constexpr (MODE == kGatedForward) {
+        v += bias4(p.bias[0], n, p.N);
+        u += bias4(p.bias[1], n, p.N);
+        const f32x4 y = activate4(v, p.act, leaky) * u;
+        if (p.C[1]) {
+            put(p.C[1] + at, n, p.N, v, p.wide);
+            put(p.C[2] + at, n, p.N, u, p.wide);
         }
-        const int which = MODE == kGatedForward ? 0 : (int)(e / one);
-        const int64_t m = (e - which * one) / lines, n = (e - which * one - m * lines) * 4;
-        const int64_t at = m * p.ldc;
-        if constexpr (MODE == kGatedForward) {
-            v += bias4(p.bias[0], n, p.N);
-            u += bias4(p.bias[1], n, p.N);
-            const f32x4 y = activate4(v, p.act, leaky) * u;
-            if (p.C[1]) {
-                put(p.C[1] + at, n, p.N, v, p.wide);
-                put(p.C[2] + at, n, p.N, u, p.wide);
-            }
-            put(p.C[0] + at, n, p.N, y, p.wide);
-        } else {
-            float* c = p.C[which] + at;
-            if (p.acc) {
+        put(p.C[0] + at, n, p.N, y, p.wide);
+    } else {
+        float* c = p.C[place.which] + at;
+        if (p.acc) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (n + i < p.N) v[i] += c[n + i];
-            }
-            put(c, n, p.N, v, p.wide);
+            for (int i = 0; i < 4; i++)
+                if (n + i < p.N) v[i] += c[n + i];
         }
+        put(c, n, p.N, v, p.wide);
     }
 }
+
+// Where the reduction is cut, whole rounds of workgroups over the chip still take whole tiles: only the rest is cut, so that few
+// sums pass through memory (4096 x 4096 -> 11008, 1376 tiles: all in two parts 3.49 ms, 1280 whole and 96 in eight 3.19).
+int whole_tiles(int64_t tiles) { return (int)(tiles / compute_units() * compute_units()); }
 
 template <int MODE, int WM, int WN, int NBM>
 int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
@@ -513,19 +525,16 @@ int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
                           "hipFuncSetAttribute(gated_gemm_kernel)"));
     const int steps = p.K / kStep * (MODE == kGatedGx ? 2 : 1);
     p.part_steps = (int)((steps + nparts - 1) / nparts + 1) / 2 * 2;
-    nparts = p.part_steps > 0 ? (steps + p.part_steps - 1) / p.part_steps : 1;
-    p.ldp = (p.N + 3) / 4 * 4;
-    if (nparts > 1) {
-        const int64_t outputs = p.M * p.ldp * (MODE == kGatedForward ? 2 : p.nwhich);
-        KAI_TRY(workspace(nparts * outputs * (int64_t)sizeof(float), &p.parts));
-    }
+    p.nparts = p.part_steps > 0 ? (steps + p.part_steps - 1) / p.part_steps : 1;
+    const int tiles = p.tiles_m * p.tiles_n * p.nwhich;
+    p.whole = p.nparts > 1 ? whole_tiles(tiles) : tiles;
+    p.cut = tiles - p.whole;
+    if (p.cut > 0) KAI_TRY(workspace((int64_t)p.nparts * p.cut * S::BM * S::BN * (int64_t)sizeof(float), &p.parts));
     p.wide = p.ldc % 4 == 0 && aligned16(p.C[0]) && aligned16(p.C[1]) && aligned16(p.C[2]);
-    const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.nwhich), (unsigned)nparts);
-    gated_gemm_kernel<MODE, WM, WN, NBM><<<grid, S::NT, S::kLds, stream>>>(p);
+    gated_gemm_kernel<MODE, WM, WN, NBM><<<(unsigned)(p.whole + p.cut * p.nparts), S::NT, S::kLds, stream>>>(p);
     KAI_TRY(check_launch("gated_gemm_kernel"));
-    if (nparts == 1) return KAI_OK;
-    const int64_t groups = (p.M * p.ldp / 4 * p.nwhich + 255) / 256, most = 16 * (int64_t)compute_units();
-    gated_parts_kernel<MODE><<<(unsigned)(groups < most ? groups : most), 256, 0, stream>>>(p, (int)nparts);
+    if (p.cut == 0) return KAI_OK;
+    gated_parts_kernel<MODE, S::BM, S::BN><<<(unsigned)(p.cut * (S::BM * S::kColumns / 1024)), 256, 0, stream>>>(p);
     return check_launch("gated_parts_kernel");
 }
 
@@ -555,9 +564,11 @@ Plan plan_of(const GatedGemm& p) {
         const int64_t tiles = (p.M + rows[t] - 1) / rows[t] * ((all_columns + columns[t] - 1) / columns[t]) * p.nwhich;
         for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
             if (parts > 1 && steps < 4 * parts) break;
-            const int64_t each = ((steps + parts - 1) / parts + 1) / 2 * 2, rounds = (tiles * parts + cu - 1) / cu;
-            double us = (MODE == kGatedForward ? fixed_forward : fixed_gradient)[t] + (double)(rounds * each) * step[t];
-            if (parts > 1) us += 4.0 + parts * (double)(p.M * all_columns * p.nwhich) * 8.0 / 1e7;
+            const int64_t each = ((steps + parts - 1) / parts + 1) / 2 * 2;
+            const int64_t whole = parts > 1 ? whole_tiles(tiles) : tiles, cut = tiles - whole;
+            const int64_t rounds = (whole + cu - 1) / cu, cut_rounds = (cut * parts + cu - 1) / cu;
+            double us = (MODE == kGatedForward ? fixed_forward : fixed_gradient)[t] + (double)(rounds * steps + cut_rounds * each) * step[t];
+            if (cut > 0) us += 4.0 + (double)(parts * cut * rows[t] * columns[t]) * 8.0 / 1e7;
             if (us < best.us) best = Plan{t, parts, us};
         }
     }

@@ -87,3 +87,31 @@ def test_gated_few_rows_both_ways(ndat, xvec, yvec):
     assert rel_fro(y.saved["up"].numpy(), up) <= REL_FRO_TOL
     assert rel_fro(y.numpy(), ACTS["swish"][0](gate) * up) <= REL_FRO_TOL
     assert np.array_equal(gated(T(x), T(wg), T(wu), None, T(bu), actfunc="swish").numpy(), y.numpy())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ndat,xvec,yvec", [(1500, 1003, 3001), (1100, 4350, 1001)])
+@pytest.mark.parametrize("acc", [False, True])
+def test_gated_more_tiles_than_compute_units(ndat, xvec, yvec, acc):
+    """Whole rounds of tiles over the chip and a cut rest, with edges in both directions: every output is written once."""
+    rng = np.random.default_rng(ndat)
+    x = rng.standard_normal((ndat, xvec)).astype(np.float32)
+    wg, wu = ((rng.uniform(-1, 1, (yvec, xvec)) * xvec ** -0.5).astype(np.float32) for _ in range(2))
+    gy = rng.standard_normal((ndat, yvec)).astype(np.float32)
+    T = Tensor.from_numpy
+    tx, twg, twu, tgy = T(x), T(wg), T(wu), T(gy)
+    y = gated(tx, twg, twu, actfunc="swish", keep=True)
+    gate, up = x.astype(np.float64) @ wg.T, x.astype(np.float64) @ wu.T
+    act, slope = ACTS["swish"]
+    assert rel_fro(y.saved["gate"].numpy(), gate) <= REL_FRO_TOL
+    assert rel_fro(y.saved["up"].numpy(), up) <= REL_FRO_TOL
+    assert rel_fro(y.numpy(), act(gate) * up) <= REL_FRO_TOL
+    g32, u32 = (y.saved[n].numpy().astype(np.float64) for n in ("gate", "up"))
+    gg, gu = gy * u32 * slope(g32), gy * act(g32)
+    start = 2.0 if acc else np.nan                # a gradient that is not added to is not read
+    out = {"x": T(np.full(x.shape, start)), "wg": T(np.full(wg.shape, start)), "wu": T(np.full(wu.shape, start))}
+    VMath.gated_backward(0, out["x"].ptr, out["wg"].ptr, out["wu"].ptr, None, None, None, tgy.ptr, twg.ptr, twu.ptr, tx.ptr,
+                         y.saved["gate"].ptr, y.saved["up"].ptr, yvec, ndat, xvec, y.saved["actfunc"], None, acc)
+    want = {"x": gg @ wg + gu @ wu, "wg": gg.T @ x, "wu": gu.T @ x}
+    for n, t in out.items():
+        assert rel_fro(t.numpy(), want[n] + (2.0 if acc else 0.0)) <= REL_FRO_TOL, n
