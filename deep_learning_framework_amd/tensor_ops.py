@@ -483,12 +483,41 @@ def gated_backprop(y, ygrad):
 
 # ---- a cache of keys and values (additive) -----------------------------------------------------------------
 
+def _device_ints(values, shape, device, what):
+    """32-bit integers of ``shape`` on the device, for a call: None, a DeviceBuffer that holds them, or host values, which are
+    copied there.  Anything else (an address among them) would be read as memory by the kernel and is refused."""
+    if values is None:
+        return None
+    if isinstance(values, DeviceBuffer):
+        if values.ptr is None or values.device != device or values.nbytes < 4 * _total(shape):
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, what)
+        return values
+    a = np.asarray(values)
+    if a.shape != shape or a.dtype.kind not in "iu":
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, what)
+    if a.dtype == np.uint32:
+        a = a.view(np.int32)             # words of bits
+    if np.any(a < -2 ** 31) or np.any(a >= 2 ** 31):
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, what)
+    return DeviceBuffer.from_numpy(a.astype(np.int32), device)
+
+
+def _device_counts(counts, nbat, device, what):
+    """As ``_device_ints`` for a number per sequence; one number stands for all."""
+    if counts is not None and not isinstance(counts, DeviceBuffer) and np.ndim(counts) == 0:
+        counts = np.full(nbat, counts)
+    return _device_ints(counts, (nbat,), device, what)
+
+
 class KeyValueCache:
     """Pages of keys and values on the device, a table that finds each sequence's pages, and its length.
 
     ``append`` writes the keys (turned by ``rotary``) and values of new tokens behind each sequence's own, ``attend``
     lets the new tokens' queries see them, ``accept`` moves the lengths on: after a drafted tree only the tokens that
-    were taken, whose rows the caller has appended again in order where they did not stand first."""
+    were taken, whose rows the caller has appended again in order where they did not stand first.
+
+    ``counts`` (a number, or one per sequence), ``positions`` [nbat, ntimes] and ``mask`` [nbat, ntimes, words] are host
+    integers or a DeviceBuffer of 32-bit ones."""
 
     def __init__(self, nbat, nkvhead, npiece, npagelen, nmaxpage, rotary=None, device=0):
         self.nbat, self.nkvhead, self.npiece = nbat, nkvhead, npiece
@@ -515,6 +544,8 @@ class KeyValueCache:
         if len(key.shape) != 3 or key.shape != value.shape or key.shape[0] != self.nbat or \
                 key.shape[2] != self.nkvhead * self.npiece:
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "append")
+        counts = _device_counts(counts, self.nbat, self.device, "append: counts")
+        positions = _device_ints(positions, key.shape[:2], self.device, "append: positions")
         VMath.cache_append(self.device, self.keys.ptr, self.values.ptr, key.ptr, value.ptr, self.table, self._len, counts,
                            positions, self.nbat, key.shape[1], key.shape[2], self.nkvhead, self.npiece, self.npage,
                            self.npagelen, self.nmaxpage, self.rotary)
@@ -522,6 +553,8 @@ class KeyValueCache:
     def attend(self, query, head_cnt, counts=None, mask=None, coef=None):
         if len(query.shape) != 3 or query.shape[0] != self.nbat or query.shape[2] != head_cnt * self.npiece:
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "attend")
+        counts = _device_counts(counts, self.nbat, self.device, "attend: counts")
+        mask = _device_ints(mask, query.shape[:2] + ((query.shape[1] + 31) // 32,), self.device, "attend: mask")
         y = Tensor(query.shape, self.device)
         VMath.set_zero(self.device, y.ptr, y.total_size() * 4)   # rows behind a sequence's count
         hcoef = kai.hyper(1.0 / np.sqrt(self.npiece) if coef is None else coef, self.device)
@@ -536,6 +569,7 @@ def rotate(x, head_cnt, desc, positions=None, back=False, out=None):
     if len(x.shape) != 3 or x.shape[2] % head_cnt != 0:
         raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate")
     nbat, ntimes, nvec = x.shape
+    positions = _device_ints(positions, (nbat, ntimes), x.device, "rotate: positions")
     y = out if out is not None else Tensor(x.shape, x.device)
     call = VMath.rotary_backward if back else VMath.rotary
     call(x.device, y.ptr, x.ptr, positions, nbat, ntimes, nvec, head_cnt, nvec // head_cnt, desc)

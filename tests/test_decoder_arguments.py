@@ -1,0 +1,77 @@
+"""What the tensor-level callers of a decoder block's operators refuse before an address reaches a kernel.  Tensors of device -1
+live in host memory, and the library refuses that device itself (510), so a call that passes its own checks ends there and none
+of this needs a GPU."""
+import numpy as np
+import pytest
+
+from deep_learning_framework_amd import kai
+from deep_learning_framework_amd.kai import DeviceBuffer, KaiError
+from deep_learning_framework_amd.tensor_ops import KeyValueCache, Tensor, gated, gated_backprop, rotate
+
+HOST = -1
+SHAPE, LIBRARY = 10003, 510
+
+
+def refused(code, call, *args, **kwargs):
+    with pytest.raises(KaiError) as e:
+        call(*args, **kwargs)
+    assert e.value.code == code, e.value.message
+
+
+def ints(a, device=HOST):
+    return DeviceBuffer.from_numpy(np.asarray(a, np.int32), device)
+
+
+def tensor(*shape):
+    return Tensor(shape, HOST)
+
+
+def test_counts_positions_and_masks_are_no_addresses():
+    cache = KeyValueCache(2, 1, 8, 4, 4, device=HOST)
+    k, q = tensor(2, 3, 8), tensor(2, 3, 16)
+    append = lambda **a: cache.append(k, k, **a)
+    attend = lambda **a: cache.attend(q, 2, **a)
+    d = kai.rotary_desc(8)
+    turn = lambda positions: rotate(q, 2, d, positions=positions)
+    freed = ints([1, 1])
+    freed.free()
+    for call in (append, attend):
+        for counts in (3.0, [1], [1, 2, 3], [1.5, 2.0], [[1, 2]], 2 ** 31, [True, False], "2", ints([1]), freed):
+            refused(SHAPE, call, counts=counts)
+        for counts in (None, 3, np.int64(2), [1, 3], np.array([0, 2]), ints([1, 1])):      # past their checks
+            refused(LIBRARY, call, counts=counts)
+    for positions in (4096, [0, 1, 2], np.zeros((2, 3)), np.full((2, 3), 2 ** 31), ints(np.zeros(5))):
+        refused(SHAPE, append, positions=positions)
+        refused(SHAPE, turn, positions)
+    for positions in (None, np.zeros((2, 3), np.int64), ints(np.zeros(6))):
+        refused(LIBRARY, append, positions=positions)
+        refused(LIBRARY, turn, positions)
+    for mask in (4096, np.zeros((2, 3), np.int32), np.zeros((2, 3, 2), np.int32), ints(np.zeros(5))):
+        refused(SHAPE, attend, mask=mask)
+    for mask in (None, np.full((2, 3, 1), 2 ** 32 - 1, np.uint32), np.zeros((2, 3, 1), np.int32), ints(np.zeros(6))):
+        refused(LIBRARY, attend, mask=mask)
+    other = ints([1, 1])
+    other.device = 0              # a buffer of another device than the cache's
+    refused(SHAPE, append, counts=other)
+    other.device = HOST
+
+
+@pytest.mark.gpu
+def test_host_values_reach_the_calls():
+    """Counts, positions and masks from the host give what the same values on the device give."""
+    rng = np.random.default_rng(5)
+    r = lambda *s: Tensor.from_numpy(rng.standard_normal(s).astype(np.float32))
+    k, v, q = r(2, 5, 16), r(2, 5, 16), r(2, 5, 32)
+    counts, positions = np.array([5, 2]), rng.integers(0, 9, (2, 5))
+    mask = np.zeros((2, 5, 1), np.uint32)
+    mask[:, :, 0] = [1, 3, 5, 0x8000000B, 31]
+    out = []
+    for put in (lambda a: a, lambda a: DeviceBuffer.from_numpy(a.astype(np.uint32).view(np.int32))):
+        cache = KeyValueCache(2, 1, 16, 4, 4, rotary=kai.rotary_desc(16))
+        cache.append(k, v, counts=put(counts), positions=put(positions))
+        turned = rotate(q, 2, cache.rotary, positions=put(positions))
+        out.append([turned.numpy(), cache.attend(turned, 2, counts=put(counts), mask=put(mask)).numpy()])
+    for a, b in zip(*out):
+        assert np.array_equal(a, b)
+    cache.append(k, v, counts=2)
+    assert np.all(cache.attend(q, 2, counts=2).numpy()[:, 2:] == 0)
