@@ -565,9 +565,11 @@ class KeyValueCache:
 
 
 def rotate(x, head_cnt, desc, positions=None, back=False, out=None):
-    """kai_rotary (``back``: kai_rotary_backward) of ``[nbat, ntimes, nvec]``; ``out`` may be ``x``."""
-    if len(x.shape) != 3 or x.shape[2] % head_cnt != 0:
+    """kai_rotary (``back``: kai_rotary_backward) of ``[nbat, ntimes, nvec]``; ``out`` has the shape of ``x`` and may be it."""
+    if len(x.shape) != 3 or head_cnt < 1 or x.shape[2] % head_cnt != 0:
         raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate")
+    if out is not None and (out.shape != x.shape or out.device != x.device):
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate: out")
     nbat, ntimes, nvec = x.shape
     positions = _device_ints(positions, (nbat, ntimes), x.device, "rotate: positions")
     y = out if out is not None else Tensor(x.shape, x.device)

@@ -56,6 +56,19 @@ def test_counts_positions_and_masks_are_no_addresses():
     other.device = HOST
 
 
+def test_rotate_writes_into_its_own_shape_only():
+    x, d = tensor(2, 3, 16), kai.rotary_desc(8)
+    for out in (tensor(2, 3, 8), tensor(1, 3, 16), tensor(6, 16), tensor(2, 16, 3)):
+        refused(SHAPE, rotate, x, 2, d, out=out)
+    elsewhere = tensor(2, 3, 16)
+    elsewhere.device = 0
+    refused(SHAPE, rotate, x, 2, d, out=elsewhere)
+    for heads in (0, -2, 3):
+        refused(SHAPE, rotate, x, heads, d)
+    for out in (None, x, tensor(2, 3, 16)):
+        refused(LIBRARY, rotate, x, 2, d, out=out)
+
+
 @pytest.mark.gpu
 def test_host_values_reach_the_calls():
     """Counts, positions and masks from the host give what the same values on the device give."""
