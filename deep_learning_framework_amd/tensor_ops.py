@@ -468,8 +468,10 @@ def gated(x, wg, wu, bg=None, bu=None, actfunc="swish", leaky_alpha=None, keep=F
 
 
 def gated_backprop(y, ygrad):
-    """The gradients of ``gated`` by name: x, wg, wu and, where there are biases, bg and bu."""
+    """The gradients of ``gated`` (with ``keep``) by name: x, wg, wu and, where there are biases, bg and bu."""
     s = y.saved
+    if s.get("op") != "gated" or ygrad.shape != y.shape or ygrad.device != y.device:
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, "gated_backprop")
     yvec, xvec = s["wg"].shape
     ndat = _total(s["x"].shape[:-1])
     dev = y.device

@@ -69,6 +69,20 @@ def test_rotate_writes_into_its_own_shape_only():
         refused(LIBRARY, rotate, x, 2, d, out=out)
 
 
+def test_gated_backprop_takes_a_gradient_of_the_result():
+    y = tensor(5, 4)
+    y.saved = {"op": "gated", "x": tensor(5, 3), "wg": tensor(4, 3), "wu": tensor(4, 3), "bg": None, "bu": None, "gate": tensor(5, 4),
+               "up": tensor(5, 4), "actfunc": 8, "leaky_alpha": None}
+    for shape in ((5, 3), (4, 4), (5,), (4, 5), (20,)):
+        refused(SHAPE, gated_backprop, y, tensor(*shape))
+    refused(LIBRARY, gated_backprop, y, tensor(5, 4))
+    refused(SHAPE, gated_backprop, tensor(5, 4), tensor(5, 4))       # of a result that kept nothing
+    x, w = tensor(5, 3), tensor(4, 3)
+    refused(SHAPE, gated, x, w, tensor(3, 3))
+    refused(SHAPE, gated, tensor(5, 4), w, w)
+    refused(SHAPE, gated, x, w, w, tensor(3))
+
+
 @pytest.mark.gpu
 def test_host_values_reach_the_calls():
     """Counts, positions and masks from the host give what the same values on the device give."""
