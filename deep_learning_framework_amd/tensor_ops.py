@@ -534,7 +534,10 @@ class KeyValueCache:
     def accept(self, counts):
         """Each sequence is ``counts`` (a number, or one per sequence) tokens longer.  The lengths change where they stand,
         for recorded graphs name the place, and behind all that still reads them."""
-        longer = self.lengths + np.asarray(counts, np.int32)
+        counts = np.asarray(counts)
+        if counts.dtype.kind not in "iu" and counts.size:
+            raise KaiError(VERR_BAD_SHAPE_TENSOR, "accept")
+        longer = self.lengths.astype(np.int64) + counts.astype(np.int64)
         if longer.shape != (self.nbat,) or np.any(longer < 0) or np.any(longer > self.npagelen * self.nmaxpage):
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "accept")
         kai.synchronize()

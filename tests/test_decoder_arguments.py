@@ -83,6 +83,18 @@ def test_gated_backprop_takes_a_gradient_of_the_result():
     refused(SHAPE, gated, x, w, w, tensor(3))
 
 
+def test_accept_takes_whole_numbers(monkeypatch):
+    monkeypatch.setattr(kai, "synchronize", lambda: None)
+    cache = KeyValueCache(2, 1, 8, 4, 4, device=HOST)
+    cache.accept(3)
+    for counts in (1.7, [0.5, 1.0], [True, True], 2 ** 32 + 1, [2 ** 32, 0], -2 ** 32, 14, [-4, 0], [1, 1, 1], [[1, 1]]):
+        with pytest.raises((KaiError, ValueError, OverflowError)):
+            cache.accept(counts)
+        assert list(cache.lengths) == [3, 3] and list(cache._len.to_numpy(2, np.int32)) == [3, 3]
+    cache.accept([13, -3])
+    assert list(cache._len.to_numpy(2, np.int32)) == [16, 0] and cache.lengths.dtype == np.int32
+
+
 @pytest.mark.gpu
 def test_host_values_reach_the_calls():
     """Counts, positions and masks from the host give what the same values on the device give."""
