@@ -516,7 +516,8 @@ class KeyValueCache:
 
     ``append`` writes the keys (turned by ``rotary``) and values of new tokens behind each sequence's own, ``attend``
     lets the new tokens' queries see them, ``accept`` moves the lengths on: after a drafted tree only the tokens that
-    were taken, whose rows the caller has appended again in order where they did not stand first.
+    were taken, whose rows the caller has appended again in order where they did not stand first.  Tokens that find no room
+    are refused where the counts are known here; counts in a DeviceBuffer are not looked at, and what is too many is dropped.
 
     ``counts`` (a number, or one per sequence), ``positions`` [nbat, ntimes] and ``mask`` [nbat, ntimes, words] are host
     integers or a DeviceBuffer of 32-bit ones."""
@@ -549,7 +550,12 @@ class KeyValueCache:
         if len(key.shape) != 3 or key.shape != value.shape or key.shape[0] != self.nbat or \
                 key.shape[2] != self.nkvhead * self.npiece:
             raise KaiError(VERR_BAD_SHAPE_TENSOR, "append")
+        held = counts
         counts = _device_counts(counts, self.nbat, self.device, "append: counts")
+        if not isinstance(held, DeviceBuffer):
+            new = np.clip(key.shape[1] if held is None else held, 0, key.shape[1])
+            if np.any(self.lengths + new > self.npagelen * self.nmaxpage):
+                raise KaiError(VERR_BAD_SHAPE_TENSOR, "append: more tokens than the sequence's pages hold")
         positions = _device_ints(positions, key.shape[:2], self.device, "append: positions")
         VMath.cache_append(self.device, self.keys.ptr, self.values.ptr, key.ptr, value.ptr, self.table, self._len, counts,
                            positions, self.nbat, key.shape[1], key.shape[2], self.nkvhead, self.npiece, self.npage,

@@ -95,6 +95,17 @@ def test_accept_takes_whole_numbers(monkeypatch):
     assert list(cache._len.to_numpy(2, np.int32)) == [16, 0] and cache.lengths.dtype == np.int32
 
 
+def test_append_refuses_what_finds_no_room(monkeypatch):
+    monkeypatch.setattr(kai, "synchronize", lambda: None)
+    cache, k = KeyValueCache(2, 1, 8, 4, 4, device=HOST), tensor(2, 3, 8)
+    cache.accept([14, 0])
+    for counts in (None, 3, 4, [3, 0], np.array([3, 1])):
+        refused(SHAPE, cache.append, k, k, counts=counts)
+    for counts in (2, [2, 3], [-1, 5], ints([3, 3])):        # the last is the device's to clip
+        refused(LIBRARY, cache.append, k, k, counts=counts)
+    refused(SHAPE, KeyValueCache(2, 1, 8, 1, 2, device=HOST).append, k, k)
+
+
 @pytest.mark.gpu
 def test_host_values_reach_the_calls():
     """Counts, positions and masks from the host give what the same values on the device give."""
