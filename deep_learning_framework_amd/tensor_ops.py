@@ -199,8 +199,12 @@ class Tensor:
         six calls between the projections, and the gradient of the probabilities is never formed).  ``g["x"]`` is the gradient of the tensor the operator was called on:
         zero, plus the gradient of each of key / query / value that IS that tensor (self-attention,
         vtensor.cpp:3168-3195).  The reference's set_zero there passes an element count where bytes are meant
-        and clears a quarter of the buffer; the whole buffer is cleared here."""
+        and clears a quarter of the buffer; the whole buffer is cleared here.  The reference's key gradient takes the
+        scores' gradient by the output row; with ``rotary``, which the reference has not, it is the derivative, gS^T . Q,
+        and the separate calls run with ``fused`` too, for that product reads all of gS."""
         s = self.saved
+        turned = s["rotary"] is not None
+        fused = fused and not turned
         nbat, ntimes, nvec = self.shape
         nhead = s["head_cnt"]
         npiece = nvec // nhead
@@ -228,9 +232,14 @@ class Tensor:
             VMath.softmax_direct_on_axis_backward(dev, g["probs"].ptr, s["probs"].ptr, nbat, ntimes, nhead, s["coef"])
             if s["mask"]:
                 VMath.set_mh_attention_mask(dev, g["probs"].ptr, nbat, ntimes, nhead, False)
-            VMath.mult_on_heads_backward(dev, g["K"].ptr, g["probs"].ptr, s["Q"].ptr, nbat, ntimes, nvec, nhead, npiece)
+            if turned:
+                VMath.mix_values_backward_value(dev, g["K"].ptr, s["Q"].ptr, g["probs"].ptr, nbat, ntimes, nvec, nhead,
+                                                npiece)
+            else:
+                VMath.mult_on_heads_backward(dev, g["K"].ptr, g["probs"].ptr, s["Q"].ptr, nbat, ntimes, nvec, nhead,
+                                             npiece)
             VMath.mult_on_heads_backward(dev, g["Q"].ptr, g["probs"].ptr, s["K"].ptr, nbat, ntimes, nvec, nhead, npiece)
-        if s["rotary"] is not None:
+        if turned:
             rotate(g["K"], nhead, s["rotary"], back=True, out=g["K"])
             rotate(g["Q"], nhead, s["rotary"], back=True, out=g["Q"])
         VMath.add_bias_backward_b(dev, g["Kb"].ptr, g["K"].ptr, n, nvec, False)
