@@ -13,6 +13,7 @@
 #include "elementwise.h"
 #include "gemm_host.h"
 #include "kai_common.h"
+#include "scratch_book.h"
 
 namespace kai {
 
@@ -36,32 +37,6 @@ int check_launch(const char* kernel_name) { return check_hip(hipGetLastError(), 
 namespace {
 constexpr int kMaxDevices = 64;
 std::mutex g_ws_mutex;
-// Per device: one scratch buffer per STREAM that calls of the library have been enqueued on (the stream a thread
-// set with kai_set_stream; the null stream counts as one), so that calls on different streams of a device never
-// share partial sums, and the smaller buffers that grown ones replaced.  A replaced buffer is only retired: kernels
-// already enqueued that use it stay valid, and growing needs neither a wait for the device nor a hipFree (which
-// waits for the device, too).  Retired buffers are released at the library's own synchronisation points, when the
-// device is idle anyway (kai_device_synchronize, kai_shutdown) -- except those that were handed out while a stream
-// capture was active: a recorded graph keeps the address and may be replayed at any later time, so they stay until
-// kai_shutdown.  Growth at least doubles the size, so the retired buffers of a stream together are smaller than
-// its current one.
-struct StreamScratch {
-    hipStream_t stream = nullptr;
-    void* ptr = nullptr;
-    int64_t bytes = 0;
-    bool in_graph = false;     // handed out during a capture
-};
-struct RetiredScratch {
-    void* ptr;
-    int64_t bytes;
-    bool in_graph;
-};
-struct DeviceScratch {
-    std::vector<StreamScratch> streams;
-    std::vector<RetiredScratch> retired;
-    int64_t retired_bytes = 0;
-    int64_t growths = 0;
-};
 DeviceScratch g_ws[kMaxDevices];
 int g_cu_count[kMaxDevices] = {};
 // bytes at the front of the scratch that an enclosing call of this thread holds (ScratchHold)
@@ -90,26 +65,10 @@ int grow_scratch(DeviceScratch& d, StreamScratch& s, int64_t need, bool capturin
     if (want < kScratchMin) want = kScratchMin;
     void* fresh = nullptr;
     KAI_TRY(check_hip(hipMalloc(&fresh, (size_t)want), "hipMalloc(scratch)"));
-    if (s.ptr) {
-        d.retired.push_back(RetiredScratch{s.ptr, s.bytes, s.in_graph});
-        d.retired_bytes += s.bytes;
-    }
-    s.ptr = fresh;
-    s.bytes = want;
-    s.in_graph = false;
-    d.growths++;
+    d.replace(s, fresh, want);
     return KAI_OK;
 }
 
-// the device is idle: every retired buffer that no recorded graph may still name goes back
-void release_retired(DeviceScratch& d) {
-    std::vector<RetiredScratch> kept;
-    for (const RetiredScratch& r : d.retired) {
-        if (r.in_graph || hipFree(r.ptr) != hipSuccess) kept.push_back(r);
-        else d.retired_bytes -= r.bytes;
-    }
-    d.retired.swap(kept);
-}
 }  // namespace
 
 int workspace(int64_t bytes, float** out) {
@@ -121,9 +80,7 @@ int workspace(int64_t bytes, float** out) {
     const bool capturing = stream_is_capturing(st);
     std::lock_guard<std::mutex> lock(g_ws_mutex);
     DeviceScratch& d = g_ws[dev];
-    StreamScratch* s = nullptr;
-    for (StreamScratch& e : d.streams)
-        if (e.stream == st) s = &e;
+    StreamScratch* s = d.find(st);
     if (s == nullptr) {
         if (d.streams.size() >= kMaxScratchStreams)
             return fail(KAI_ERR_INVALID_ARGUMENT, "workspace: more than 64 streams of one device have asked for scratch memory; "
@@ -139,8 +96,19 @@ int workspace(int64_t bytes, float** out) {
     return KAI_OK;
 }
 
-ScratchHold::ScratchHold(int64_t bytes) : previous_(tl_ws_held) { tl_ws_held += (bytes + 255) / 256 * 256; }
-ScratchHold::~ScratchHold() { tl_ws_held = previous_; }
+ScratchHold::ScratchHold(int64_t bytes) : previous_(tl_ws_held), stream_(current_stream()) {
+    if (bytes <= 0 || hipGetDevice(&device_) != hipSuccess || device_ < 0 || device_ >= kMaxDevices) device_ = -1;
+    tl_ws_held += (bytes + 255) / 256 * 256;
+    if (device_ < 0) return;
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    g_ws[device_].hold(stream_, 1);
+}
+ScratchHold::~ScratchHold() {
+    tl_ws_held = previous_;
+    if (device_ < 0) return;
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    g_ws[device_].hold(stream_, -1);
+}
 
 int compute_units() {
     int dev = 0;
@@ -174,12 +142,20 @@ static int release_workspaces() {
     return rc;
 }
 
-// after a successful wait for the current device
-static void release_retired_of_current_device() {
+// Waits for the current device and releases what it had retired before: see scratch_book.h.
+static int wait_and_release_retired() {
     int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return;
+    std::vector<RetiredScratch> idle;
+    if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < kMaxDevices) {
+        std::lock_guard<std::mutex> lock(g_ws_mutex);
+        idle = g_ws[dev].take_idle();
+    }
+    const int rc = check_hip(hipDeviceSynchronize(), "hipDeviceSynchronize");
+    if (idle.empty()) return rc;
     std::lock_guard<std::mutex> lock(g_ws_mutex);
-    release_retired(g_ws[dev]);
+    for (const RetiredScratch& r : idle)
+        if (rc != KAI_OK || hipFree(r.ptr) != hipSuccess) g_ws[dev].put_back(r);
+    return rc;
 }
 
 static bool act_is_elementwise(int act) { return act >= KAI_ACT_NONE && act <= KAI_ACT_SWISH; }
@@ -205,11 +181,8 @@ int kai_device_count(int* count) {
 
 int kai_set_device(int device) { return check_hip(hipSetDevice(device), "hipSetDevice"); }
 
-int kai_device_synchronize(void) {
-    KAI_TRY(check_hip(hipDeviceSynchronize(), "hipDeviceSynchronize"));
-    release_retired_of_current_device();   // the device is idle: scratch buffers that grown ones replaced go back
-    return KAI_OK;
-}
+// the device is idle then: scratch buffers that grown ones replaced go back
+int kai_device_synchronize(void) { return wait_and_release_retired(); }
 
 int kai_set_stream(void* hip_stream) {
     tl_stream = reinterpret_cast<hipStream_t>(hip_stream);

@@ -35,7 +35,8 @@ int check_launch(const char* kernel_name);
 int workspace(int64_t bytes, float** out);
 // While an object of this type lives, workspace() calls of the same thread return memory BEHIND the first
 // `bytes` bytes of the scratch: for a call that keeps data in the scratch across inner calls which may ask
-// for scratch themselves.
+// for scratch themselves.  An inner call may replace the buffer by a larger one: the held one is not released before the
+// object is gone.
 class ScratchHold {
 public:
     explicit ScratchHold(int64_t bytes);
@@ -45,6 +46,8 @@ public:
 
 private:
     int64_t previous_;
+    hipStream_t stream_;
+    int device_ = -1;      // of the buffer that is held; -1: none
 };
 // number of compute units of the current device (cached)
 int compute_units();
