@@ -575,15 +575,6 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentio
         a.y[row * c.npiece + d] = sum == 0.0f ? 0.0f : (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) / sum;
 }
 
-int parts_buffer(Parts* parts, int64_t rows, int npiece) {
-    float* buf = nullptr;
-    const int64_t slots = (int64_t)parts->nsplit * rows;
-    KAI_TRY(workspace(slots * (npiece + 2) * (int64_t)sizeof(float), &buf));
-    parts->ml = reinterpret_cast<float2*>(buf);
-    parts->acc = buf + 2 * slots;
-    return KAI_OK;
-}
-
 template <int VW, int NR>
 int launch_tiled(const CacheAttentionArgs& a, const Parts& parts, int64_t row_tiles, hipStream_t stream) {
     const CachePages& c = a.pages;
@@ -605,9 +596,8 @@ int launch_tiled_rows(const CacheAttentionArgs& a, const Parts& parts, int nr, i
     return launch_tiled<VW, 4>(a, parts, row_tiles, stream);
 }
 
-bool tiled_applies(const CacheAttentionArgs& a) {
-    const int np = a.pages.npiece;
-    return np == 32 || np == 64 || np == 80 || np == 96 || np == 128;
+bool tiled_applies(int npiece) {
+    return npiece == 32 || npiece == 64 || npiece == 80 || npiece == 96 || npiece == 128;
 }
 
 int launch_tiled_any(const CacheAttentionArgs& a, const Parts& parts, int nr, int64_t row_tiles, hipStream_t stream) {
@@ -622,12 +612,11 @@ int launch_tiled_any(const CacheAttentionArgs& a, const Parts& parts, int nr, in
 
 }  // namespace
 
-int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
-    const CachePages& c = a.pages;
-    const int64_t rows = c.nbat * c.ntimes * a.nhead;
+int cache_attention_plan(const CachePages& c, int nhead, CacheAttentionPlan* plan) {
+    const int64_t rows = c.nbat * c.ntimes * nhead;
     const int64_t reach = c.page * c.nmaxpage;
-    const bool tiled = tiled_applies(a);
-    const int64_t shared_rows = c.ntimes * (a.nhead / c.nkvhead);      // of a key head
+    const bool tiled = tiled_applies(c.npiece);
+    const int64_t shared_rows = c.ntimes * (nhead / c.nkvhead);      // of a key head
     const int64_t cu = compute_units();
     // parts down to a tile of 32 keys for each wave
     const int64_t tiles = (reach + 127) / 128, most = tiles < 1 ? 1 : tiles > kMaxParts ? kMaxParts : tiles;
@@ -650,15 +639,33 @@ int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
     if (c.nbat > 1 && reach >= 2 * nsplit * 512) nsplit *= 2;
     if (nsplit > most) nsplit = most;
     if (nsplit < 1) nsplit = 1;
-    Parts parts{nullptr, nullptr, (int)nsplit};
-    if (nsplit > 1) KAI_TRY(parts_buffer(&parts, rows, c.npiece));
-    if (tiled) {
-        KAI_TRY(launch_tiled_any(a, parts, nr, row_tiles, stream));
+    plan->row_tile = tiled ? 16 * nr : 0;
+    plan->row_tiles = row_tiles;
+    plan->groups = groups;
+    plan->nsplit = (int)nsplit;
+    plan->scratch = nsplit > 1 ? nsplit * rows * (c.npiece + 2) * (int64_t)sizeof(float) : 0;
+    return KAI_OK;
+}
+
+int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream) {
+    const CachePages& c = a.pages;
+    const int64_t rows = c.nbat * c.ntimes * a.nhead;
+    CacheAttentionPlan plan;
+    KAI_TRY(cache_attention_plan(c, a.nhead, &plan));
+    Parts parts{nullptr, nullptr, plan.nsplit};
+    if (plan.nsplit > 1) {
+        float* buf = nullptr;
+        KAI_TRY(workspace(plan.scratch, &buf));
+        parts.ml = reinterpret_cast<float2*>(buf);
+        parts.acc = buf + 2 * plan.nsplit * rows;
+    }
+    if (plan.row_tile > 0) {
+        KAI_TRY(launch_tiled_any(a, parts, plan.row_tile / 16, plan.row_tiles, stream));
     } else {
-        cache_attention_rows_kernel<<<dim3((unsigned)groups, (unsigned)nsplit), 256, 0, stream>>>(a, parts);
+        cache_attention_rows_kernel<<<dim3((unsigned)plan.groups, (unsigned)plan.nsplit), 256, 0, stream>>>(a, parts);
         KAI_TRY(check_launch("cache_attention_rows_kernel"));
     }
-    if (nsplit == 1) return KAI_OK;
+    if (plan.nsplit == 1) return KAI_OK;
     cache_attention_join_kernel<<<(unsigned)rows, 256, 0, stream>>>(a, parts);
     return check_launch("cache_attention_join_kernel");
 }

@@ -66,6 +66,13 @@ struct CacheAttentionArgs {
     const float* hcoef;
 };
 int launch_cache_attention(const CacheAttentionArgs& a, hipStream_t stream);
+// How it runs this geometry (host arithmetic; the pages' pointers are not read).
+struct CacheAttentionPlan {
+    int row_tile;           // rows of a key head that a workgroup takes, 0: a wave takes a row
+    int nsplit;             // parts of the keys
+    int64_t row_tiles, groups, scratch;   // tiles of a key head's rows; workgroups of a part; bytes
+};
+int cache_attention_plan(const CachePages& c, int nhead, CacheAttentionPlan* plan);
 
 struct GatedArgs {
     float* y;               // forward
@@ -99,6 +106,8 @@ struct GatedGradArgs {
 };
 // gx (+)= ggate . wg + gup . wu, gwg (+)= ggate^T . x, gwu (+)= gup^T . x
 int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream);
+// how the forward (0), the gradient of x (1) or those of both weights (2) run with 16-byte aligned operands, as text
+std::string gated_plan_text(int which, int64_t yvec, int64_t ndat, int64_t xvec);
 
 // ggate = gy * up * act'(gate), gup = gy * act(gate), [nrow, ncol] each, and their column sums gbg, gbu (+= with acc; null:
 // not wanted)

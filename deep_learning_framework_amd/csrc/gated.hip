@@ -135,7 +135,7 @@ int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float
     return check_launch("gated_bias_kernel");
 }
 
-int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
+static GatedGemm forward_product(const GatedArgs& a) {
     GatedGemm p{};
     p.A[0] = a.x; p.B[0] = a.wg; p.B[1] = a.wu;
     p.C[0] = a.y; p.C[1] = a.gate; p.C[2] = a.up;
@@ -144,8 +144,14 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
     p.M = a.ndat; p.N = a.yvec; p.K = (int)a.xvec;
     p.lda = p.ldb = a.xvec; p.ldc = a.yvec;
     p.nwhich = 1;
+    return p;
+}
+static bool tiled_forward(const GatedArgs& a, const GatedGemm& p) { return a.ndat > 32 && gated_gemm_applies(kGatedForward, p); }
+
+int launch_gated_forward(const GatedArgs& a, hipStream_t stream) {
+    const GatedGemm p = forward_product(a);
     if (gated_rows_pays(a)) return launch_gated_rows(a, stream);
-    if (a.ndat > 32 && gated_gemm_applies(kGatedForward, p)) return launch_gated_gemm(kGatedForward, p, stream);
+    if (tiled_forward(a, p)) return launch_gated_gemm(kGatedForward, p, stream);
     // both products, then the activation and the product; the pre-activations in the caller's buffers or in scratch
     const int64_t n = a.ndat * a.yvec;
     float* gate = a.gate;
@@ -177,16 +183,38 @@ static bool split_pays(int mode, const GatedGemm& p, int64_t ndat) {
     return gated_gemm_us(mode, p) < 7.0 + flops / 65e6;
 }
 
-int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
+static GatedGemm x_product(const GatedGradArgs& a) {
     GatedGemm p{};
     p.A[0] = a.ggate; p.A[1] = a.gup;
+    p.B[0] = a.wg; p.B[1] = a.wu;
+    p.C[0] = a.gx;
+    p.M = a.ndat; p.N = a.xvec; p.K = (int)a.yvec;
+    p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
     p.acc = a.acc;
     p.nwhich = 1;
+    return p;
+}
+static GatedGemm weight_product(const GatedGradArgs& a) {
+    GatedGemm p{};
+    p.A[0] = a.ggate; p.A[1] = a.gup;
+    p.B[0] = a.x;
+    p.C[0] = a.gwg; p.C[1] = a.gwu;
+    p.M = a.yvec; p.N = a.xvec; p.K = (int)a.ndat;
+    p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
+    p.acc = a.acc;
+    p.nwhich = 2;
+    if (a.gwg == nullptr || a.gwu == nullptr) {
+        p.nwhich = 1;
+        p.C[0] = a.gwg ? a.gwg : a.gwu;
+        p.C[1] = nullptr;
+        p.A[0] = a.gwg ? a.ggate : a.gup;
+    }
+    return p;
+}
+
+int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
     if (a.gx) {
-        p.B[0] = a.wg; p.B[1] = a.wu;
-        p.C[0] = a.gx;
-        p.M = a.ndat; p.N = a.xvec; p.K = (int)a.yvec;
-        p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
+        const GatedGemm p = x_product(a);
         if (split_pays(kGatedGx, p, a.ndat)) {
             KAI_TRY(launch_gated_gemm(kGatedGx, p, stream));
         } else {
@@ -195,21 +223,28 @@ int launch_gated_gradients(const GatedGradArgs& a, hipStream_t stream) {
         }
     }
     if (a.gwg == nullptr && a.gwu == nullptr) return KAI_OK;
-    p.B[0] = a.x; p.B[1] = nullptr;
-    p.M = a.yvec; p.N = a.xvec; p.K = (int)a.ndat;
-    p.lda = a.yvec; p.ldb = p.ldc = a.xvec;
-    p.C[0] = a.gwg; p.C[1] = a.gwu;
-    p.nwhich = 2;
-    if (a.gwg == nullptr || a.gwu == nullptr) {
-        p.nwhich = 1;
-        p.C[0] = a.gwg ? a.gwg : a.gwu;
-        p.C[1] = nullptr;
-        p.A[0] = a.gwg ? a.ggate : a.gup;
-    }
+    const GatedGemm p = weight_product(a);
     if (split_pays(kGatedGw, p, a.ndat)) return launch_gated_gemm(kGatedGw, p, stream);
     if (a.gwg) KAI_TRY(kai_matmul_backward_w(0, a.gwg, a.ggate, a.x, a.yvec, a.ndat, a.xvec, a.acc));
     if (a.gwu) KAI_TRY(kai_matmul_backward_w(0, a.gwu, a.gup, a.x, a.yvec, a.ndat, a.xvec, a.acc));
     return KAI_OK;
+}
+
+std::string gated_plan_text(int which, int64_t yvec, int64_t ndat, int64_t xvec) {
+    static float there;      // of outputs that are wanted; nothing is read
+    GatedArgs f{};
+    f.yvec = yvec; f.ndat = ndat; f.xvec = xvec;
+    GatedGradArgs g{};
+    g.gwg = g.gwu = &there;
+    g.yvec = yvec; g.ndat = ndat; g.xvec = xvec;
+    const int mode = which == 0 ? kGatedForward : which == 1 ? kGatedGx : kGatedGw;
+    const GatedGemm p = which == 0 ? forward_product(f) : which == 1 ? x_product(g) : weight_product(g);
+    if (which == 0 && gated_rows_pays(f)) return "rows";
+    if (which == 0 ? !tiled_forward(f, p) : !split_pays(mode, p, ndat)) return "separate";
+    const GatedGemmPlan plan = gated_gemm_plan(mode, p);
+    std::string text = "tiles " + std::to_string(plan.rows) + " x " + std::to_string(plan.columns) + ", " + std::to_string(plan.whole) + " whole";
+    if (plan.cut > 0) text += ", " + std::to_string(plan.cut) + " in " + std::to_string(plan.parts) + " parts";
+    return text + ", scratch " + std::to_string(plan.scratch);
 }
 
 }  // namespace kai

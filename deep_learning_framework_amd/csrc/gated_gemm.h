@@ -28,6 +28,13 @@ struct GatedGemm {
 bool gated_gemm_applies(int mode, const GatedGemm& p);
 // what the products would take, as the choice of their tiles estimates it
 double gated_gemm_us(int mode, const GatedGemm& p);
+// the plan itself: tiles of rows x columns of the products (forward: of gate and up together), those taken whole and those
+// whose reduction is cut into parts, and the bytes of scratch that the parts take
+struct GatedGemmPlan {
+    int rows, columns, whole, cut, parts;
+    int64_t scratch;
+};
+GatedGemmPlan gated_gemm_plan(int mode, const GatedGemm& p);
 int launch_gated_gemm(int mode, const GatedGemm& p, hipStream_t stream);
 
 }  // namespace kai

@@ -513,23 +513,33 @@ __global__ __launch_bounds__(256) void gated_parts_kernel(GatedGemm p) {
 // sums pass through memory (4096 x 4096 -> 11008, 1376 tiles: all in two parts 3.49 ms, 1280 whole and 96 in eight 3.19).
 int whole_tiles(int64_t tiles) { return (int)(tiles / compute_units() * compute_units()); }
 
-template <int MODE, int WM, int WN, int NBM>
-int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
-    using S = Shape<MODE, WM, WN, NBM>;
-    p.tiles_m = (int)((p.M + S::BM - 1) / S::BM);
-    p.tiles_n = (int)((p.N + S::kColumns - 1) / S::kColumns);
+// Tiles of rows x columns of the output, and how their reduction is cut.
+template <int MODE>
+void place_tiles(GatedGemm& p, int rows, int columns, int64_t nparts) {
+    p.tiles_m = (int)((p.M + rows - 1) / rows);
+    p.tiles_n = (int)((p.N + columns - 1) / columns);
     p.run = 8;
-    if (S::kLds > 64 * 1024)
-        KAI_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_gemm_kernel<MODE, WM, WN, NBM>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds),
-                          "hipFuncSetAttribute(gated_gemm_kernel)"));
     const int steps = p.K / kStep * (MODE == kGatedGx ? 2 : 1);
     p.part_steps = (int)((steps + nparts - 1) / nparts + 1) / 2 * 2;
     p.nparts = p.part_steps > 0 ? (steps + p.part_steps - 1) / p.part_steps : 1;
     const int tiles = p.tiles_m * p.tiles_n * p.nwhich;
     p.whole = p.nparts > 1 ? whole_tiles(tiles) : tiles;
     p.cut = tiles - p.whole;
-    if (p.cut > 0) KAI_TRY(workspace((int64_t)p.nparts * p.cut * S::BM * S::BN * (int64_t)sizeof(float), &p.parts));
+}
+
+int64_t parts_bytes(int64_t nparts, int64_t cut, int64_t rows, int64_t columns) {
+    return nparts * cut * rows * columns * (int64_t)sizeof(float);
+}
+
+template <int MODE, int WM, int WN, int NBM>
+int launch_shape(GatedGemm p, int64_t nparts, hipStream_t stream) {
+    using S = Shape<MODE, WM, WN, NBM>;
+    place_tiles<MODE>(p, S::BM, S::kColumns, nparts);
+    if (S::kLds > 64 * 1024)
+        KAI_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_gemm_kernel<MODE, WM, WN, NBM>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds),
+                          "hipFuncSetAttribute(gated_gemm_kernel)"));
+    if (p.cut > 0) KAI_TRY(workspace(parts_bytes(p.nparts, p.cut, S::BM, S::BN), &p.parts));
     p.wide = p.ldc % 4 == 0 && aligned16(p.C[0]) && aligned16(p.C[1]) && aligned16(p.C[2]);
     gated_gemm_kernel<MODE, WM, WN, NBM><<<(unsigned)(p.whole + p.cut * p.nparts), S::NT, S::kLds, stream>>>(p);
     KAI_TRY(check_launch("gated_gemm_kernel"));
@@ -552,9 +562,11 @@ struct Plan {
     double us = 1e30;
 };
 
+constexpr int kTileRows[4] = {64, 128, 256, 256}, kTileColumns[4] = {128, 128, 128, 256};
+
 template <int MODE>
 Plan plan_of(const GatedGemm& p) {
-    constexpr int rows[4] = {64, 128, 256, 256}, columns[4] = {128, 128, 128, 256};
+    const int(&rows)[4] = kTileRows, (&columns)[4] = kTileColumns;
     constexpr double step[4] = {0.42, 0.70, 1.25, 2.35};
     constexpr double fixed_forward[4] = {7.7, 12.0, 15.0, 19.0}, fixed_gradient[4] = {5.2, 6.5, 8.0, 14.0};
     const int64_t all_columns = MODE == kGatedForward ? 2 * p.N : p.N, cu = compute_units();
@@ -573,6 +585,15 @@ Plan plan_of(const GatedGemm& p) {
         }
     }
     return best;
+}
+
+template <int MODE>
+GatedGemmPlan full_plan(GatedGemm p) {
+    const Plan plan = plan_of<MODE>(p);
+    const int rows = kTileRows[plan.tile], columns = kTileColumns[plan.tile];
+    place_tiles<MODE>(p, rows, MODE == kGatedForward ? columns / 2 : columns, plan.parts);
+    const int parts = p.cut > 0 ? p.nparts : 1;
+    return GatedGemmPlan{rows, columns, p.whole, p.cut, parts, p.cut > 0 ? parts_bytes(parts, p.cut, rows, columns) : 0};
 }
 
 template <int MODE>
@@ -598,6 +619,11 @@ bool gated_gemm_applies(int mode, const GatedGemm& p) {
 
 double gated_gemm_us(int mode, const GatedGemm& p) {
     return mode == kGatedForward ? plan_of<kGatedForward>(p).us : mode == kGatedGx ? plan_of<kGatedGx>(p).us : plan_of<kGatedGw>(p).us;
+}
+
+GatedGemmPlan gated_gemm_plan(int mode, const GatedGemm& p) {
+    if (mode == kGatedForward) return full_plan<kGatedForward>(p);
+    return mode == kGatedGx ? full_plan<kGatedGx>(p) : full_plan<kGatedGw>(p);
 }
 
 int launch_gated_gemm(int mode, const GatedGemm& p, hipStream_t stream) {

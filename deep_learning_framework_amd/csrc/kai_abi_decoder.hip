@@ -1,6 +1,7 @@
 // extern "C" surface of the operators of a decoder block (declared in include/kai_hip.h): argument checks and the
 // host arithmetic in front of the launchers of decoder_ops.h.
 #include <cmath>
+#include <cstdio>
 
 #include "decoder_ops.h"
 #include "elementwise.h"
@@ -220,6 +221,38 @@ int kai_gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* 
     a.wg = pwg; a.wu = pwu; a.x = px;
     a.yvec = yvec; a.ndat = ndat; a.xvec = xvec; a.acc = acc != 0;
     return launch_gated_gradients(a, current_stream());
+}
+
+int kai_cache_attention_plan(int64_t nbat, int64_t ntimes, int64_t nhead, int64_t nkvhead, int64_t npiece, int64_t npagelen,
+                             int64_t nmaxpage, char* out, int buflen) {
+    KAI_REQUIRE_PTR(out);
+    KAI_REQUIRE(buflen > 0, KAI_ERR_INVALID_ARGUMENT, "buflen <= 0");
+    KAI_TRY(check_head_rows(__func__, nbat, ntimes, kMaxWidth, nhead, npiece));
+    const int some = 0;      // the table is not read
+    CachePages c{};
+    KAI_TRY(cache_pages(__func__, &c, &some, nullptr, nullptr, nbat, ntimes, nkvhead, npiece, 1, npagelen, nmaxpage));
+    KAI_REQUIRE(npiece <= kMaxAttentionPiece, KAI_ERR_INVALID_ARGUMENT, "npiece above 256");
+    std::string text = "nothing";
+    if (nbat > 0 && ntimes > 0 && nhead > 0 && npiece > 0) {
+        KAI_REQUIRE(nkvhead > 0 && nhead % nkvhead == 0, KAI_ERR_INVALID_ARGUMENT, "nhead must be a multiple of nkvhead");
+        KAI_REQUIRE(nbat * ntimes <= kMaxAttentionRows / nhead, KAI_ERR_INVALID_ARGUMENT, "nbat * ntimes * nhead above 2^25");
+        CacheAttentionPlan plan;
+        KAI_TRY(cache_attention_plan(c, (int)nhead, &plan));
+        text = plan.row_tile > 0 ? "tiles of " + std::to_string(plan.row_tile) + " rows" : std::string("a wave a row");
+        text += ", " + std::to_string(plan.nsplit) + (plan.nsplit == 1 ? " part" : " parts") + ", scratch " + std::to_string(plan.scratch);
+    }
+    snprintf(out, (size_t)buflen, "%s", text.c_str());
+    return KAI_OK;
+}
+
+int kai_gated_plan(int which, int64_t yvec, int64_t ndat, int64_t xvec, char* out, int buflen) {
+    KAI_REQUIRE_PTR(out);
+    KAI_REQUIRE(buflen > 0, KAI_ERR_INVALID_ARGUMENT, "buflen <= 0");
+    KAI_REQUIRE(which >= 0 && which <= 2, KAI_ERR_INVALID_ARGUMENT, "which must be 0..2");
+    KAI_REQUIRE_DIM(yvec); KAI_REQUIRE_DIM(ndat); KAI_REQUIRE_DIM(xvec);
+    const std::string text = yvec == 0 || ndat == 0 ? "nothing" : gated_plan_text(which, yvec, ndat, xvec);
+    snprintf(out, (size_t)buflen, "%s", text.c_str());
+    return KAI_OK;
 }
 
 }  // extern "C"

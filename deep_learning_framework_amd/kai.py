@@ -93,6 +93,8 @@ SIGNATURES = {
     "kai_cache_attention": [_INT] + [_F] * 8 + [_I64] * 9 + [_F],
     "kai_gated_forward": [_INT] + [_F] * 8 + [_I64] * 3 + [_INT, _F],
     "kai_gated_backward": [_INT] + [_F] * 12 + [_I64] * 3 + [_INT, _F, _INT],
+    "kai_cache_attention_plan": [_I64] * 7 + [ctypes.c_char_p, _INT],
+    "kai_gated_plan": [_INT] + [_I64] * 3 + [ctypes.c_char_p, _INT],
 }
 
 ACT = {"none": 0, "relu": 1, "leaky": 2, "sigmoid": 3, "tanh": 4, "gelu": 5, "selu": 6, "mish": 7, "swish": 8,
@@ -547,3 +549,18 @@ class VMath:
                                                  yvec, ndat, xvec, actFunc, hLeakyAlpha, acc)
         if rc:
             _ck(rc)
+
+    @staticmethod
+    def cache_attention_plan(nbat, ntimes, nhead, nkvhead, npiece, npagelen, nmaxpage):
+        """How ``cache_attention`` would run this geometry, as text (host arithmetic only)."""
+        buf = ctypes.create_string_buffer(128)
+        _ck(load().kai_cache_attention_plan(nbat, ntimes, nhead, nkvhead, npiece, npagelen, nmaxpage, buf, 128))
+        return buf.value.decode()
+
+    @staticmethod
+    def gated_plan(which, yvec, ndat, xvec):
+        """How ``which`` = "forward", "x" or "weights" (gradients) of the gated projection would run, as text."""
+        buf = ctypes.create_string_buffer(128)
+        code = {"forward": 0, "x": 1, "weights": 2}[which]
+        _ck(load().kai_gated_plan(code, yvec, ndat, xvec, buf, 128))
+        return buf.value.decode()

@@ -480,6 +480,17 @@ int kai_gated_backward(int device, float* pgx, float* pgwg, float* pgwu, float* 
                        const float* pup, int64_t yvec, int64_t ndat, int64_t xvec, int actFunc, const float* hLeakyAlpha,
                        int acc);
 
+/* Write into `out` how these geometries run, as text.  Host arithmetic only, nothing is launched and no GPU is needed.  For
+ * maintainers, tests, and callers who size the scratch.
+ * kai_cache_attention: "tiles of 16 | 32 | 64 rows, P parts, scratch B" (head sizes 32, 64, 80, 96 and 128; rows of one key head
+ * share a tile) or "a wave a row, P parts, scratch B", B in bytes.
+ * kai_gated_plan, with 16-byte aligned operands, which = 0: kai_gated_forward, 1: the gradient of x, 2: those of both
+ * weights: "rows" (up to 32 rows in one launch), "tiles R x C, N whole[, M in P parts], scratch B", or "separate": products
+ * of the dense layer (kai_gemm_plan tells theirs) beside element-wise launches. */
+int kai_cache_attention_plan(int64_t nbat, int64_t ntimes, int64_t nhead, int64_t nkvhead, int64_t npiece, int64_t npagelen,
+                             int64_t nmaxpage, char* out, int buflen);
+int kai_gated_plan(int which, int64_t yvec, int64_t ndat, int64_t xvec, char* out, int buflen);
+
 #ifdef __cplusplus
 }
 #endif
