@@ -115,9 +115,11 @@ int launch_gated_activation_backward(float* ggate, float* gup, float* gbg, float
     const int64_t chunk = (nrow + chunks - 1) / chunks;
     chunks = (nrow + chunk - 1) / chunk;
     float* sums = nullptr;
-    // no scratch to be had (the stream is being captured and the buffer would have to grow): the sums read the gradients again
+    // no scratch to be had (the stream is being captured and the buffer would have to grow), or more than a product may ask: the
+    // sums read the gradients again
     const bool wanted = gbg || gbu;
-    const bool fused = wanted && workspace(2 * chunks * ncol * (int64_t)sizeof(float), &sums) == KAI_OK;
+    const int64_t sums_bytes = 2 * chunks * ncol * (int64_t)sizeof(float);
+    const bool fused = wanted && sums_bytes <= kProductScratchMax && workspace(sums_bytes, &sums) == KAI_OK;
     if (wanted && !fused) {
         sums = nullptr;
         clear_error();

@@ -578,6 +578,7 @@ Plan plan_of(const GatedGemm& p) {
             if (parts > 1 && steps < 4 * parts) break;
             const int64_t each = ((steps + parts - 1) / parts + 1) / 2 * 2;
             const int64_t whole = parts > 1 ? whole_tiles(tiles) : tiles, cut = tiles - whole;
+            if (parts > 1 && parts_bytes(parts, cut, rows[t], columns[t]) > kProductScratchMax) break;
             const int64_t rounds = (whole + cu - 1) / cu, cut_rounds = (cut * parts + cu - 1) / cu;
             double us = (MODE == kGatedForward ? fixed_forward : fixed_gradient)[t] + (double)(rounds * steps + cut_rounds * each) * step[t];
             if (cut > 0) us += 4.0 + (double)(parts * cut * rows[t] * columns[t]) * 8.0 / 1e7;

@@ -22,7 +22,7 @@ static int64_t tiles_of(int64_t M, int64_t N, int64_t nbatch, int64_t t) {
 constexpr int64_t kSplitFromK = 512;
 constexpr int64_t kSplitMinK = 64;
 constexpr int64_t kSplitMax = 16;
-constexpr int64_t kSplitScratchMax = 64ll << 20;   // bytes of partial sums a product may ask of the library scratch
+constexpr int64_t kSplitScratchMax = kProductScratchMax;
 
 static int launch_layout(const GemmParams& p, bool a_kc, bool b_kc, int64_t nbatch, int tile, hipStream_t stream) {
     if (a_kc && b_kc) return launch_gemm_kc_kc(p, nbatch, tile, stream);

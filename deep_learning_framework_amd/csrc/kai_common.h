@@ -55,6 +55,7 @@ int compute_units();
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int64_t kMaxDim = (1ll << 31) - 1;
+constexpr int64_t kProductScratchMax = 64ll << 20;   // bytes of partial sums that a product may ask of the library scratch
 
 }  // namespace kai
 

@@ -87,10 +87,10 @@ int kai_shutdown(void);
 /* Makes the current device's scratch at least `bytes` large now, so that later calls find it and allocate
  * nothing: for callers that record calls into a HIP graph (a call whose scratch would have to grow while its
  * stream is being captured fails with KAI_ERR_GPU) or that cannot tolerate an allocation inside a step.  A
- * product never asks for more than 64 MiB of partial sums; kai_attention_forward outside the fused head sizes
- * asks for nbat*ntimes*ntimes*nhead floats on top; kai_cache_attention for what its declaration says;
- * kai_gated_backward without a work buffer for 2*ndat*yvec floats, kai_gated_forward with null pgate at most for as many,
- * and either for up to 16 parts of its products' results.  Growing never waits for the device: the smaller buffer is
+ * product never asks for more than 64 MiB of partial sums, those of kai_gated_forward and kai_gated_backward with their bias
+ * sums among them; kai_attention_forward outside the fused head sizes asks for nbat*ntimes*ntimes*nhead floats on top;
+ * kai_gated_backward without a work buffer for 2*ndat*yvec floats on top, rounded up to whole 256 bytes, kai_gated_forward with
+ * null pgate at most for as many; kai_cache_attention for what kai_cache_attention_plan says, never as much as 64 MiB.  Growing never waits for the device: the smaller buffer is
  * kept until kai_shutdown, so work in flight and recorded graphs stay valid.  No counterpart in the reference. */
 int kai_reserve_scratch(int64_t bytes);
 /* Current size of the current device's scratch, how many times it was allocated or grown since the last
@@ -458,7 +458,7 @@ int kai_cache_append(int device, float* pcK, float* pcV, const float* pK, const 
  * npiece is at most 256, nbat * ntimes * nhead at most 2^25, nbat * nkvhead at most 2^23.  A row that sees no key, or none
  * whose score is above minus infinity, gives zeros; what stands at keys that a row does not see (NaN included) does not
  * reach it.  The keys are cut into parts whose results meet in the library scratch (nbat * ntimes * nhead * (npiece + 2)
- * floats a part, up to 256 parts where there are few rows). */
+ * floats a part, up to 256 parts where there are few rows, below 64 MiB in all: kai_cache_attention_plan tells). */
 int kai_cache_attention(int device, float* py, const float* pQ, const float* pcK, const float* pcV, const int* ppage,
                         const int* plen, const int* pcount, const int* pmask, int64_t nbat, int64_t ntimes, int64_t nvec,
                         int64_t nhead, int64_t nkvhead, int64_t npiece, int64_t npage, int64_t npagelen, int64_t nmaxpage,

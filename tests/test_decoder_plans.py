@@ -1,5 +1,7 @@
 """How the decoder block's calls choose to run a geometry: host arithmetic, no GPU (256 compute units are assumed without one)."""
 import ctypes
+import random
+import re
 
 import pytest
 
@@ -36,6 +38,25 @@ def test_cache_attention_plans(geometry, expected):
 ])
 def test_gated_plans(which, yvec, ndat, xvec, expected):
     assert VMath.gated_plan(which, yvec, ndat, xvec) == expected
+
+
+def test_scratch_stays_below_what_a_product_may_ask():
+    """Callers reserve 64 MiB for a product's parts before they record a graph."""
+    rng = random.Random(5)
+    size = lambda low, high: int(round(2 ** rng.uniform(low, high)))
+    shapes = [(11008, 4096, 4096), (18371, 4849, 14840), (193, 193, 4096)]
+    for yvec, ndat, xvec in shapes + [(size(6, 15), size(6, 14), size(6, 15)) for _ in range(4000)]:
+        for which in ("forward", "x", "weights"):
+            text = VMath.gated_plan(which, yvec, ndat, xvec)
+            if text.startswith("tiles"):
+                tile = re.match(r"tiles (\d+) x (\d+), (\d+) whole(?:, (\d+) in (\d+) parts)?, scratch (\d+)$", text)
+                rows, columns, whole, cut, parts, scratch = (int(v or 0) for v in tile.groups())
+                assert scratch == 4 * rows * columns * cut * parts <= 64 << 20, (which, yvec, ndat, xvec, text)
+    for _ in range(4000):
+        nkv, group = rng.choice([1, 2, 3, 8, 12, 64]), rng.choice([1, 2, 5, 8])
+        geometry = (size(0, 8), size(0, 8), nkv * group, nkv, rng.choice([32, 64, 80, 96, 128, 20, 256, 1]), size(0, 10), size(0, 14))
+        text = VMath.cache_attention_plan(*geometry)
+        assert int(text.rsplit(" ", 1)[1]) < 64 << 20, (geometry, text)
 
 
 def test_plans_check_their_arguments():
