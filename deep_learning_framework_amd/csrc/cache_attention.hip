@@ -4,8 +4,9 @@
 //
 // with online statistics: a running maximum m, the sum l of exp(s_j - m) and the sum of exp(s_j - m) v_j, all in
 // 32 bits; a row that sees nothing gives zeros.  Few rows meet many keys, so the keys of a sequence are cut into
-// parts that run as separate workgroups; cache_attention_join_kernel adds the parts,
-//   y = sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s.
+// parts that run as separate workgroups; cache_attention_join_kernel adds the parts' own results y_s = acc_s / l_s,
+//   y = sum_s w_s y_s,   w_s = e^(m_s - M) l_s / sum_s e^(m_s - M) l_s,
+// a weighted mean, which stays finite where the sums of large values would not.
 //
 // Bound: HBM (the keys and values once, 8 bytes an element pair) while a key head has few rows: 32 sequences x 1 token of 32 heads
 // of 128 on 8 key heads over up to 4096 keys 135 us = 5.4 TB/s.  From some 50 rows of a key head on the matrix cores and the
@@ -28,7 +29,7 @@ constexpr int kMaxParts = 256;   // a thread of the joining workgroup each
 constexpr int kKeyStep = 32;     // a part of a sequence's keys is a whole number of these
 
 struct Parts {
-    float* acc;      // [nsplit][rows][npiece], not yet divided
+    float* acc;      // [nsplit][rows][npiece]: the parts' results
     float2* ml;      // [nsplit][rows]: maximum, sum
     int nsplit;
 };
@@ -91,13 +92,14 @@ __device__ __forceinline__ unsigned eight_seen(const int* mask, int64_t ntimes, 
     return s < 0 ? (bits << -s | ((1u << -s) - 1)) & 0xFFu : bits;
 }
 
-// Results of a row: straight to y, or the part's sums.
+// Results of a row: straight to y, or the part's.
 __device__ __forceinline__ int64_t slot_of(const Parts& parts, int64_t rows, int64_t row, int split) {
     return (int64_t)split * rows + row;
 }
 
 // One row (b, t, h) over the keys [begin, end), a wave with its lanes along the head: any head size up to kMaxPiece, any
-// alignment, plain fp32 sums, and only what the row sees is read into them.
+// alignment, plain fp32 sums, and only what the row sees is read into them.  Where sums pass the largest float (up to 2^30 values
+// below 2^128), a second pass with the weights times 2^-32 forms them anew, and only them: smaller ones beside them would lose bits.
 __device__ void attend_row(const CacheAttentionArgs& a, const Parts& parts, const Sequence& seq, int b, int t, int h, int split,
                            int begin, int end) {
     const int lane = threadIdx.x & (kWave - 1);
@@ -106,53 +108,63 @@ __device__ void attend_row(const CacheAttentionArgs& a, const Parts& parts, cons
     const int np = c.npiece, kvh = h / (a.nhead / c.nkvhead);
     const int64_t width = (int64_t)c.nkvhead * np;
     const float coef = a.hcoef ? *a.hcoef : 0.0f;
-    float q[kMaxPiece / kWave], acc[kMaxPiece / kWave];
+    float* out = a.y + row * np;
+    float2* ml = nullptr;
+    if (parts.nsplit > 1) {
+        const int64_t slot = slot_of(parts, c.nbat * c.ntimes * a.nhead, row, split);
+        ml = parts.ml + slot;
+        out = parts.acc + slot * np;
+    }
+    float q[kMaxPiece / kWave];
 #pragma unroll
     for (int i = 0; i < kMaxPiece / kWave; i++) {
         const int d = lane + i * kWave;
         q[i] = d < np ? a.q[bt * a.ldq + (int64_t)h * np + d] : 0.0f;
-        acc[i] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = begin; j < end; j++) {
-        if (j >= seq.len && !sees_new(a.mask, c.ntimes, b, t, j - seq.len)) continue;
-        const int64_t at = row_of_key(c, b, j);
-        if (at < 0) continue;
-        const int64_t base = at * width + (int64_t)kvh * np;
-        float s = 0.0f;
+    float down = 1.0f;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        float acc[kMaxPiece / kWave] = {};
+        float m = -INFINITY, l = 0.0f;
+        for (int j = begin; j < end; j++) {
+            if (j >= seq.len && !sees_new(a.mask, c.ntimes, b, t, j - seq.len)) continue;
+            const int64_t at = row_of_key(c, b, j);
+            if (at < 0) continue;
+            const int64_t base = at * width + (int64_t)kvh * np;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kMaxPiece / kWave; i++) {
+                const int d = lane + i * kWave;
+                if (d < np) s = fmaf(q[i], a.ck[base + d], s);
+            }
+#pragma unroll
+            for (int w = 1; w < kWave; w *= 2) s += __shfl_xor(s, w);
+            s *= coef;
+            const float top = fmaxf(m, s);
+            // the first key, or a maximum of minus infinity so far: nothing to rescale
+            const float scale = m == top ? 1.0f : expf(m - top);
+            const float p = s == -INFINITY ? 0.0f : expf(s - top);
+            l = l * scale + p;
+            const float weight = p * down;
+#pragma unroll
+            for (int i = 0; i < kMaxPiece / kWave; i++) {
+                const int d = lane + i * kWave;
+                if (d < np && s != -INFINITY) acc[i] = acc[i] * scale + weight * a.cv[base + d];
+            }
+            m = top;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / (l * down);
+        bool passed = false;
 #pragma unroll
         for (int i = 0; i < kMaxPiece / kWave; i++) {
             const int d = lane + i * kWave;
-            if (d < np) s = fmaf(q[i], a.ck[base + d], s);
+            const bool over = !(fabsf(acc[i]) <= kLargestFinite);
+            if (d < np && (pass == 0 || !(fabsf(out[d]) <= kLargestFinite))) out[d] = acc[i] * inv;
+            passed |= over;
         }
-#pragma unroll
-        for (int w = 1; w < kWave; w *= 2) s += __shfl_xor(s, w);
-        s *= coef;
-        const float top = fmaxf(m, s);
-        // the first key, or a maximum of minus infinity so far: nothing to rescale
-        const float scale = m == top ? 1.0f : expf(m - top);
-        const float p = s == -INFINITY ? 0.0f : expf(s - top);
-        l = l * scale + p;
-#pragma unroll
-        for (int i = 0; i < kMaxPiece / kWave; i++) {
-            const int d = lane + i * kWave;
-            if (d < np && s != -INFINITY) acc[i] = acc[i] * scale + p * a.cv[base + d];
-        }
-        m = top;
-    }
-    float* out = a.y + row * np;
-    float inv = 1.0f;
-    if (parts.nsplit > 1) {
-        const int64_t slot = slot_of(parts, c.nbat * c.ntimes * a.nhead, row, split);
-        if (lane == 0) parts.ml[slot] = make_float2(m, l);
-        out = parts.acc + slot * np;
-    } else {
-        inv = l == 0.0f ? 0.0f : 1.0f / l;
-    }
-#pragma unroll
-    for (int i = 0; i < kMaxPiece / kWave; i++) {
-        const int d = lane + i * kWave;
-        if (d < np) out[d] = acc[i] * inv;
+        if (ml && lane == 0) *ml = make_float2(m, l);
+        if (!(l <= kLargestFinite) || !__any(passed)) break;     // a NaN among the scores: every element is one
+        down = 0x1p-32f;
     }
 }
 
@@ -482,7 +494,7 @@ __global__ __launch_bounds__(256, VW * NR > 16 ? 1 : 2) void cache_attention_til
     }
     __syncthreads();
     // Infinities and NaN in the cache come out as NaN in any row of the tile, those that do not see them too where others
-    // do: the rows are then done again one by one.
+    // do, and sums of large values as infinities: the rows are then done again one by one.
     float test = 0.0f;
     const int i = threadIdx.x & 3, rn = threadIdx.x >> 2 & 15, rg = wave;
 #pragma unroll 1
@@ -505,12 +517,11 @@ __global__ __launch_bounds__(256, VW * NR > 16 ? 1 : 2) void cache_attention_til
         const int t = row / group, h = kvh * group + (row - t * group);
         const int64_t at = ((int64_t)b * c.ntimes + t) * a.nhead + h;
         float* out = a.y + at * np;
-        float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (parts.nsplit > 1) {
             const int64_t slot = slot_of(parts, c.nbat * c.ntimes * a.nhead, at, split);
             if (threadIdx.x % 4 == 0 && rg == 0) parts.ml[slot] = make_float2(top, sum);
             out = parts.acc + slot * np;
-            inv = 1.0f;
         }
         test += sum * 0.0f;
 #pragma unroll
@@ -528,8 +539,8 @@ __global__ __launch_bounds__(256, VW * NR > 16 ? 1 : 2) void cache_attention_til
     }
 }
 
-// A workgroup for a row: y = sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s over the parts that saw a key.  Each thread
-// finds a part's weight; then the four waves take every fourth part, the lanes along the head, and meet in LDS.
+// A workgroup for a row: y = sum_s w_s y_s over the parts that saw a key.  Each thread finds a part's weight; then the four waves
+// take every fourth part, the lanes along the head, and meet in LDS.
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentionArgs a, Parts parts) {
     __shared__ float weight[kMaxParts], scratch[8], sums[4][kMaxPiece];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -547,14 +558,15 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentio
     __syncthreads();
     top = fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
     // a part that saw no key has a sum of 0; one whose scores are all NaN has a NaN, and no maximum that weighs it
-    const float mine = ml.y == 0.0f ? 0.0f : ml.y != ml.y ? ml.y : ml.x == top ? 1.0f : expf(ml.x - top);
-    weight[threadIdx.x] = mine;
-    float sum = mine == 0.0f ? 0.0f : mine * ml.y;
+    const float mine = ml.y == 0.0f ? 0.0f : ml.y != ml.y ? ml.y : ml.x == top ? ml.y : ml.y * expf(ml.x - top);
+    float sum = mine;
 #pragma unroll
     for (int w = 1; w < kWave; w *= 2) sum += __shfl_xor(sum, w);
     if (lane == 0) scratch[4 + wave] = sum;
     __syncthreads();
     sum = scratch[4] + scratch[5] + scratch[6] + scratch[7];
+    weight[threadIdx.x] = sum == 0.0f ? 0.0f : mine / sum;
+    __syncthreads();
     float acc[kMaxPiece / kWave] = {};
 #pragma unroll 4
     for (int s = wave; s < parts.nsplit; s += 4) {
@@ -563,16 +575,13 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(CacheAttentio
 #pragma unroll
         for (int i = 0; i < kMaxPiece / kWave; i++) {
             const int d = lane + i * kWave;
-            const float v = d < c.npiece ? from[d] : 0.0f;
-            // a weight that has vanished takes a sum that passed the largest float away, but no NaN
-            if (w != 0.0f || v != v) acc[i] += w * v;
+            acc[i] += w * (d < c.npiece ? from[d] : 0.0f);
         }
     }
 #pragma unroll
     for (int i = 0; i < kMaxPiece / kWave; i++) sums[wave][lane + i * kWave] = acc[i];
     __syncthreads();
-    for (int d = threadIdx.x; d < c.npiece; d += 256)
-        a.y[row * c.npiece + d] = sum == 0.0f ? 0.0f : (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) / sum;
+    for (int d = threadIdx.x; d < c.npiece; d += 256) a.y[row * c.npiece + d] = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
 }
 
 template <int VW, int NR>

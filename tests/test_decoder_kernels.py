@@ -103,6 +103,38 @@ def test_attention_tiles_unseen_keys_and_missing_pages(case, npiece):
         assert np.all(np.abs(got[1, :rest] - want[1, :rest]) <= room[1, :rest])
 
 
+LARGE = [
+    # npiece, ntimes, nhead, nkv, page, pages a sequence, lens, plan
+    (64, 3, 4, 2, 64, 3, [150], "tiles of 16 rows, 2 parts"), (64, 3, 4, 2, 128, 1, [100], "tiles of 16 rows, 1 part,"),
+    (128, 23, 16, 4, 128, 128, [1100], "tiles of 64 rows"), (32, 7, 32, 8, 100, 80, [1500], "tiles of 32 rows"),
+    (20, 3, 4, 2, 64, 20, [900], "a wave a row, 10 parts"), (20, 3, 4, 2, 128, 1, [100], "a wave a row, 1 part,"),
+    (256, 2, 2, 1, 64, 20, [900], "a wave a row, 10 parts"),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_attention_of_large_values(case):
+    """Values whose sum passes the largest float: their weighted mean does not, and small ones beside them keep their bits."""
+    npiece, ntimes, nhead, nkv, page, most, lens, plan = LARGE[case]
+    rng = np.random.default_rng(500 + case)
+    c = wide_table(_attention_case(rng, 1, ntimes, nhead, nkv, npiece, page, lens, None, False), most)
+    assert plan_of(c).startswith(plan), plan_of(c)
+    c["cv"] = (rng.uniform(0.5, 1.0, c["cv"].shape) * 2e38).astype(np.float32)
+    c["cv"][..., 1::2] *= np.float32(1e-38)
+    c["cv"][..., 3::4] *= np.float32(1e-24)
+    c["cv"][..., 2::8] *= -1
+    got = _attend(c)
+    want, _ = _expected(c)
+    room = 0 * want
+    for d in range(npiece):                      # the bound of each column by its own values
+        room[..., d] = np.abs(c["cv"].reshape(-1, nkv, npiece)[:, :, d]).max()
+    # relative to the largest value: the scores' errors as in test_decoder_ops.py (coef sum |q k| is below 30), and a rounding a key
+    keys = lens[0] + ntimes
+    off = (npiece + 2) * 2.0 ** -24 * 30
+    assert np.all(np.abs(got - want) <= room * (2 * np.expm1(off) + (keys + 24) * 2.0 ** -24))
+    assert np.abs(got).max() > 1e38
+
+
 # ---- the gated projection's tiles -------------------------------------------------------------------------------------------
 
 GATED_TILES = [
