@@ -35,9 +35,10 @@ int rotary_params(const char* who, const kai_rotary_desc* desc, int64_t npiece, 
     if (desc->nrot == 0) return KAI_OK;
     // comparisons that a NaN fails as well
     if (!(desc->base > 0.0 && std::isfinite(desc->base))) return bad("base must be positive and finite");
-    if (!std::isfinite(desc->magnitude)) return bad("magnitude must be finite");
+    if (!std::isfinite((float)desc->magnitude)) return bad("magnitude must be finite, in 32 bits too");
     const bool scaled = desc->scaling != KAI_ROTARY_SCALE_NONE;
-    if (scaled && !(desc->factor > 0.0 && std::isfinite(desc->factor))) return bad("factor must be positive and finite");
+    if (scaled && !(desc->factor > 0.0 && std::isfinite(desc->factor) && std::isfinite(1.0 / desc->factor)))
+        return bad("factor must be positive and finite, and so must its inverse");
     double log2_base = std::log2(desc->base);
     switch (desc->scaling) {
     case KAI_ROTARY_SCALE_NONE:
@@ -58,11 +59,15 @@ int rotary_params(const char* who, const kai_rotary_desc* desc, int64_t npiece, 
         r.low = desc->low_turns;
         r.inv_span = 1.0 / (desc->high_turns - desc->low_turns);
         r.trained_turns = desc->trained * 0.15915494309189533577;
+        if (!(r.inv_span > 0.0 && std::isfinite(r.inv_span))) return bad("low_turns and high_turns too near or too far apart");
         break;
     default:
         return bad("unknown scaling");
     }
     r.step = -2.0 * log2_base / (double)desc->nrot;
+    // the fastest pair's angle at position 2^31 has to be a number (a base below 1 turns the last pair fastest)
+    const double fastest = std::fmax(0.0, r.step * (double)(desc->nrot / 2 - 1)) + std::fmax(0.0, std::log2(r.inv_factor));
+    if (!(fastest + 31.0 < 1000.0)) return bad("angles out of range");
     r.magnitude = (float)desc->magnitude;
     r.nrot = (int)desc->nrot;
     r.pairs = desc->layout == KAI_ROTARY_PAIRS;

@@ -408,7 +408,7 @@ int kai_attention_backward(int device, float* pgQ, float* pgK, float* pgV, const
 /* How positions turn the heads, host memory, read during the call.  Pair i of the nrot rotated elements at the front
  * of a head (0 <= nrot <= npiece, even, at most 512) turns by f_i = base^(-2i / nrot) radians a position, scaled for
  * contexts longer than the trained one; cosine and sine are multiplied by `magnitude`.  Fields that a scaling does
- * not name are not read. */
+ * not name are not read.  A description whose angles are no numbers in 64 bits, or its magnitude none in 32, is refused. */
 typedef struct kai_rotary_desc {
     int64_t nrot;
     int32_t layout;

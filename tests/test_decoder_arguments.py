@@ -106,6 +106,22 @@ def test_append_refuses_what_finds_no_room(monkeypatch):
     refused(SHAPE, KeyValueCache(2, 1, 8, 1, 2, device=HOST).append, k, k)
 
 
+def test_rotary_descriptions_whose_angles_are_no_numbers():
+    """Each field is a number by itself, but not what is computed from it: cosines of infinity were written as NaN."""
+    nothing = lambda d: kai.VMath.rotary(0, None, None, None, 0, 3, 512, 1, 512, d)      # no rows: the description alone counts
+    parts = dict(scaling="parts", factor=2.0, trained=10.0)
+    for d in (kai.rotary_desc(8, magnitude=1e39), kai.rotary_desc(8, magnitude=-1e300), kai.rotary_desc(512, base=1e-305), kai.rotary_desc(8, base=1e-300, scaling="linear", factor=1e-200),
+              kai.rotary_desc(8, scaling="linear", factor=5e-324), kai.rotary_desc(8, scaling="linear", factor=1e-300),
+              kai.rotary_desc(4, scaling="base", factor=1e-308), kai.rotary_desc(8, **dict(parts, factor=1e-300)),
+              kai.rotary_desc(8, low_turns=0.0, high_turns=5e-324, **parts),
+              kai.rotary_desc(8, low_turns=-1.7e308, high_turns=1.7e308, **parts)):
+        refused(LIBRARY, nothing, d)
+    for d in (kai.rotary_desc(8, base=0.5), kai.rotary_desc(8, base=1e-300), kai.rotary_desc(8, base=1e300), kai.rotary_desc(8, magnitude=3e38),
+              kai.rotary_desc(8, scaling="linear", factor=1e-3), kai.rotary_desc(8, scaling="base", factor=1e300),
+              kai.rotary_desc(8, low_turns=1.0, high_turns=1.0 + 2.0 ** -40, **parts)):
+        nothing(d)
+
+
 @pytest.mark.gpu
 def test_host_values_reach_the_calls():
     """Counts, positions and masks from the host give what the same values on the device give."""
