@@ -513,6 +513,12 @@ def _device_ints(values, shape, device, what):
     return DeviceBuffer.from_numpy(a.astype(np.int32), device)
 
 
+def _check_desc(desc, what):
+    """A description is a kai.rotary_desc or none: the call reads 64 bytes of host memory where it is given."""
+    if desc is not None and not isinstance(desc, kai.RotaryDesc):
+        raise KaiError(VERR_BAD_SHAPE_TENSOR, what)
+
+
 def _device_counts(counts, nbat, device, what):
     """As ``_device_ints`` for a number per sequence; one number stands for all."""
     if counts is not None and not isinstance(counts, DeviceBuffer) and np.ndim(counts) == 0:
@@ -532,6 +538,7 @@ class KeyValueCache:
     integers or a DeviceBuffer of 32-bit ones."""
 
     def __init__(self, nbat, nkvhead, npiece, npagelen, nmaxpage, rotary=None, device=0):
+        _check_desc(rotary, "KeyValueCache: rotary")
         self.nbat, self.nkvhead, self.npiece = nbat, nkvhead, npiece
         self.npagelen, self.nmaxpage, self.npage = npagelen, nmaxpage, nbat * nmaxpage
         self.rotary, self.device = rotary, device
@@ -590,6 +597,7 @@ def rotate(x, head_cnt, desc, positions=None, back=False, out=None):
         raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate")
     if out is not None and (out.shape != x.shape or out.device != x.device):
         raise KaiError(VERR_BAD_SHAPE_TENSOR, "rotate: out")
+    _check_desc(desc, "rotate: desc")
     nbat, ntimes, nvec = x.shape
     positions = _device_ints(positions, (nbat, ntimes), x.device, "rotate: positions")
     y = out if out is not None else Tensor(x.shape, x.device)

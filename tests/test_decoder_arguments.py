@@ -69,6 +69,14 @@ def test_rotate_writes_into_its_own_shape_only():
         refused(LIBRARY, rotate, x, 2, d, out=out)
 
 
+def test_a_rotary_description_is_no_address():
+    x = tensor(2, 3, 16)
+    for desc in (4096, 1.0, {"nrot": 8}, "halves"):
+        refused(SHAPE, rotate, x, 2, desc)
+        refused(SHAPE, KeyValueCache, 2, 1, 8, 4, 4, rotary=desc, device=HOST)
+    refused(LIBRARY, KeyValueCache(2, 1, 8, 4, 4, rotary=kai.rotary_desc(8), device=HOST).append, tensor(2, 3, 8), tensor(2, 3, 8))
+
+
 def test_gated_backprop_takes_a_gradient_of_the_result():
     y = tensor(5, 4)
     y.saved = {"op": "gated", "x": tensor(5, 3), "wg": tensor(4, 3), "wu": tensor(4, 3), "bg": None, "bu": None, "gate": tensor(5, 4),
