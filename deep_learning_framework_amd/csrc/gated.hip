@@ -20,7 +20,7 @@ __global__ __launch_bounds__(kThreads) void gated_activation_kernel(float* y, co
 // ggate = gy * up * act'(gate), gup = gy * act(gate) and, on the way, their column sums: a workgroup takes 64 * VEC columns of
 // `chunk` rows, a wave every fourth of them, and leaves the sums of its rows in sums[2][chunks][ncol] (null: no sums wanted).
 // Bound: HBM, five floats an element; the sums cost nothing beside that, where sums of the stored gradients would read
-// two of the five again.  2048 x 4096: 31 us = 5.4 TB/s, and 4.6 for the chunks' sums.
+// two of the five again.  2048 x 4096: 31 .. 37 us = 5.4 .. 4.5 TB/s, and 4.6 for the chunks' sums.
 template <int VEC>
 __global__ __launch_bounds__(kThreads) void gated_activation_backward_kernel(float* ggate, float* gup, float* sums, const float* gy,
                                                                              const float* gate, const float* up, int64_t nrow,

@@ -6,15 +6,15 @@
 //   gx        [M, N] = gg[M, K] . wg[K, N] + gu . wu: one reduction over both pairs, one after the other
 //   gw        gwg | gwu [M, N] = gg^T | gu^T . x, operands [K, M] and [K, N]: the two products side by side in one launch
 //
-// A workgroup stages 16 steps of its operands' rows at a time: global loads to registers one step ahead, there cut into
+// A workgroup stages 16 steps of its operands' rows at a time: global loads to registers two steps ahead, there cut into
 // three bf16 planes (which also turns a [K, rows] operand: a thread holds eight steps of one row), LDS double buffered,
 // one barrier a step.  LDS holds a plane as [half of the steps][row][8 steps]: fragments are 16-byte chunks of
 // consecutive rows, read and (but for K-contiguous operands' half chunks) written without bank conflicts.
 //
 // Bound: the matrix cores at a sixth of their bf16 rate (235 TFLOP/s of fp32 products at what large bf16 products reach, 1412),
-// with the cutting's vector instructions between them.  4096 x 4096 -> 11008 forward 3.19 ms = 232 TFLOP/s; gradients of 2048 x 1024 ->
-// 4096 177 and 178 us = 194 and 193 TFLOP/s; small products the chain of their steps (1000 x 777 -> 333 17 us and 5.4 for the
-// sums of two parts).
+// with the cutting's vector instructions between them.  4096 x 4096 -> 11008 forward 3.15 ms = 234 TFLOP/s on
+// one card, 3.47 on another; gradients of 2048 x 1024 -> 4096 173 .. 184 us each = 199 .. 187 TFLOP/s; small products the chain of
+// their steps (1000 x 777 -> 333 17 .. 18 us and 5.4 for the sums of two parts).
 //
 // What lies outside an operand reads as 0 (buffer loads end with it); the last, partial step of a K-contiguous operand is
 // masked.  Where an operand held an infinity, which the pieces turn into a NaN, sums that came out as NaN are formed again in
@@ -510,7 +510,8 @@ __global__ __launch_bounds__(256) void gated_parts_kernel(GatedGemm p) {
 }
 
 // Where the reduction is cut, whole rounds of workgroups over the chip still take whole tiles: only the rest is cut, so that few
-// sums pass through memory (4096 x 4096 -> 11008, 1376 tiles: all in two parts 3.49 ms, 1280 whole and 96 in eight 3.19).
+// sums pass through memory (4096 x 4096 -> 11008, 1376 tiles: all in two parts 3.49 ms, 1280 whole and 96 in eight 3.19; in two,
+// what 64 MiB of scratch hold, the same: 3.45, 3.47 | 3.46, 3.47 side by side on a slower card).
 int whole_tiles(int64_t tiles) { return (int)(tiles / compute_units() * compute_units()); }
 
 // Tiles of rows x columns of the output, and how their reduction is cut.

@@ -1,9 +1,12 @@
-// fp32 products on the bf16 matrix cores without losing fp32's accuracy.
+// fp32 products on the bf16 matrix cores at about fp32's accuracy.
 //
 // A float is the exact sum of three bf16: h = its upper 16 bits, m = the upper 16 bits of x - h, l = x - h - m: 8 + 8 + 8
 // bits of the 24, |m| < 2^-7 |x|, |l| < 2^-15 |x|.  Of the nine products of two such sums six are formed: hh, hm, mh, mm,
-// hl, lh.  The three left out are below 2^-21 |x y| together, and in the mean 2^-24 |x y| (towards zero): half a step of
-// fp32, what rounding a product once may cost.  The products themselves are exact in the 32-bit accumulators.
+// hl, lh.  The three left out, m l, l m and l l, have the product's own sign: a result loses up to 2^-21 of sum |x y|, always
+// towards zero.  That is 4e-8 of it on normal or uniform data (0.7 of 2^-24, the most that rounding a product once costs, there
+// with either sign), 8e-8 where x and y are spread over [1, 1 + 2^-7), 2.5e-7 .. 4.7e-7 where nearly all of their lower bits
+// are set.  The sums' own rounding is above that from some tens of terms on.  The products formed are exact in the 32-bit
+// accumulators.
 // (Pieces rounded to nearest instead would leave out 2^-26, but v_cvt_pk_bf16_f32 issues in 8 cycles where the 32-bit
 // operations here take 4 to 5: 4096 x 4096 -> 11008 3.81 ms with them, 3.67 without.)
 // v_mfma_f32_32x32x16_bf16 does 16 times the work of v_mfma_f32_32x32x2_f32 in a cycle, so six of them are 2.67 times
