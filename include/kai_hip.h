@@ -467,7 +467,9 @@ int kai_cache_attention(int device, float* py, const float* pQ, const float* pcK
 /* The gated feed-forward projection: py[ndat, yvec] = act(px . pwg^T + pbg) * (px . pwu^T + pbu), pwg and pwu
  * [yvec, xvec], the biases [yvec] or null, activation codes 0..8.  pgate and pup (both or neither) receive the two sums
  * in front of the activation and the product, which kai_gated_backward reads.  The outputs overlap neither one another
- * nor the inputs. */
+ * nor the inputs.  Products are formed from three bf16 pieces a float, as kai_cache_attention's are: of a sum of products up to
+ * 2^-21 of sum |x y| (4e-8 of it on ordinary data) is left out, towards zero; what runs as separate products
+ * (kai_gated_plan) has fp32's own rounding. */
 int kai_gated_forward(int device, float* py, float* pgate, float* pup, const float* pwg, const float* pwu,
                       const float* pbg, const float* pbu, const float* px, int64_t yvec, int64_t ndat, int64_t xvec,
                       int actFunc, const float* hLeakyAlpha);

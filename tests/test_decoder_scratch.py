@@ -27,8 +27,8 @@ def _body():
     P, V = lambda a: a.data_ptr(), kai.VMath
     stream = torch.cuda.Stream()
     # the small one takes 16 parts of 16 tiles, the large one cut its rest into 192 MiB of parts; 24 rows run as separate products,
-    # and 64 x 20000 has wide bias sums
-    for ndat, xvec, yvec in ((193, 4096, 193), (4096, 1024, 11008), (24, 4096, 11008), (64, 300, 20000)):
+    # 64 x 20000 has wide bias sums, and those of 9 million columns would pass 64 MiB: they are taken from the gradients
+    for ndat, xvec, yvec in ((193, 4096, 193), (4096, 1024, 11008), (24, 4096, 11008), (64, 300, 20000), (2, 1, 9000000)):
         gen = torch.Generator(device=dev).manual_seed(ndat)
         r = lambda *s: torch.empty(s, device=dev).normal_(generator=gen).mul_(0.05)
         x, wg, wu, gate, up, gy = r(ndat, xvec), r(yvec, xvec), r(yvec, xvec), r(ndat, yvec), r(ndat, yvec), r(ndat, yvec)
@@ -60,6 +60,10 @@ def _body():
                 torch.cuda.synchronize()
                 assert all(torch.equal(a, b) for a, b in zip(outs, want))
             assert kai.scratch_info()[1] == 1
+        sg = torch.sigmoid(gate.double())
+        for got, each in ((outs[4], gy * up * (sg + gate * sg * (1 - sg))), (outs[5], gy * gate * sg)):
+            # of ndat numbers below 0.05^2 * 6^2: as many roundings as there are terms, and some for the slope
+            assert (got - each.sum(0)).abs().max() <= (ndat + 20) * 2.0 ** -24 * each.abs().sum(0).max()
         del graph
         kai.set_stream(None)
         torch.cuda.synchronize()
