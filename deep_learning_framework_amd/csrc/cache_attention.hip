@@ -439,8 +439,8 @@ __global__ __launch_bounds__(256, VW * NR > 16 ? 1 : 2) void cache_attention_til
             }
             // a row that has seen nothing yet keeps exp(-inf - 0) = 0
             const float base = m[r] == -INFINITY ? 0.0f : m[r];
-            // e^-d as 2^(-d log2 e): the rounded product moves it by d 2^-24 of itself, which is below 0.37 * 2^-24 of the largest
-            // probability (d e^-d <= 1 / e); the instruction flushes what is below 2^-126 of that
+            // e^-d as 2^(-d log2 e): the constant and the product, rounded, move it by 2 d 2^-24 of itself at most, which is below
+            // 0.74 * 2^-24 of the largest probability (d e^-d <= 1 / e); what is below 2^-126 of that becomes 0
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = __builtin_amdgcn_exp2f((x[i] - base) * 1.4426950408889634f);
