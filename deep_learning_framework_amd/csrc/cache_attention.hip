@@ -10,7 +10,7 @@
 //
 // Bound: HBM (the keys and values once, 8 bytes an element pair) while a key head has few rows: 32 sequences x 1 token of 32 heads
 // of 128 on 8 key heads over up to 4096 keys 135 us = 5.4 TB/s.  From some 50 rows of a key head on the matrix cores and the
-// cutting of keys and values take as long as the bytes: 1 x 16 tokens over 131072 keys 279 .. 297 us = 3.8 .. 3.6 TB/s and 122 .. 115 TFLOP/s.
+// cutting of keys and values take as long as the bytes: 1 x 16 tokens over 131072 keys 276 .. 297 us = 3.9 .. 3.6 TB/s and 124 .. 115 TFLOP/s.
 // Short caches are a chain of latencies (lengths, page, keys, the joining launch): 3 x up to 61 tokens of 12 heads of 64 over up to
 // 1500 keys 22.0 us, 17.6 of them the tiled kernel's (three tiles of keys a wave) and 4.6 the join's.
 //
